@@ -601,6 +601,92 @@ int otf_emd_lds_nodes(void);
 int otf_emd_solve(int32_t nprob, const otf_emd_problem* probs, int64_t max_pivots,
                   otf_emd_info* info, otf_stream_t stream);
 
+/* ------------------------------------------------------------------------------------
+ * Layers of the fusion block that stand around the OT features (MRI_PET_OT_nojax.py:658-669,
+ * --projection-dropout): dropout, layer norm, the residual sum with both, and (below) the
+ * gated feed-forward block, each with its backward pass.
+ *
+ * dtype: OTF_F32 / OTF_F16 / OTF_BF16 of x, y, dy, dx.  Rows may have any leading dimension
+ * >= cols and any alignment of their element.  Statistics and sums are float32.
+ * rows may be 0 (nothing is written but the parameter gradients, as zeros).
+ *
+ * rng: DEVICE pointer to two int64, {seed, offset}.  The mask of an element depends on
+ *   (seed, offset, row, column, cols) alone (Philox4x32-10, 16 bits an element), so backward
+ *   makes the forward's mask again from the same two words; calls that must not share a mask
+ *   take different seeds or offsets.  A captured graph reads the words at every replay.
+ * p: 0 <= p <= 1, rounded to a multiple t of 2^-16 (p < 1 keeps t <= 65535); kept elements are
+ *   scaled by 65536 / (65536 - t), dropped ones are an exact 0 whatever they held.
+ * weight, bias: cols elements of wdtype (the input's type or OTF_F32), each may be NULL.
+ * mean, rstd: float32 a row, both or neither.                                              */
+
+/* y = [residual +] dropout(x).  The backward of x is the same call on dy without residual. */
+int otf_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy, int64_t rows,
+                int64_t cols, int32_t dtype, double p, const int64_t* rng, otf_stream_t stream);
+
+/* y = (x - mean) rstd weight + bias, rstd = 1 / sqrt(var + eps), per row. */
+int otf_layer_norm(const void* x, int64_t ldx, int32_t dtype, const void* weight, const void* bias, int32_t wdtype,
+                   double eps, int64_t rows, int64_t cols, void* y, int64_t ldy, float* mean, float* rstd,
+                   otf_stream_t stream);
+
+/* dx, and dweight / dbias (wdtype; both NULL: not computed).  Without parameter gradients the
+ * workspace may be NULL.  Deterministic: partial sums are joined in a fixed order.          */
+size_t otf_layer_norm_backward_workspace_size(int64_t rows, int64_t cols);
+int otf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                            const void* weight, int32_t wdtype, const float* mean, const float* rstd, int64_t rows,
+                            int64_t cols, void* dx, int64_t lddx, void* dweight, void* dbias, void* workspace,
+                            size_t workspace_bytes, otf_stream_t stream);
+
+/* z = residual + dropout(x) (rdtype: dtype or OTF_F32; rounded once), y = layer norm of z as
+ * stored.  residual, z: rdtype; x, y: dtype.                                               */
+int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const void* residual, int64_t ldr,
+                               int32_t rdtype, const void* weight, const void* bias, int32_t wdtype, double eps,
+                               double p, const int64_t* rng, int64_t rows, int64_t cols, void* y, int64_t ldy,
+                               void* z, int64_t ldz, float* mean, float* rstd, otf_stream_t stream);
+
+/* From dy (of y) and dz (of z, NULL: zero): dresidual = dz + LN'(dy), dx = dropout'(dresidual),
+ * dweight, dbias.  Workspace: otf_layer_norm_backward_workspace_size.                       */
+int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void* dz, int64_t lddz, const void* z,
+                                        int64_t ldz, int32_t dtype, int32_t rdtype, const void* weight,
+                                        int32_t wdtype, const float* mean, const float* rstd, double p,
+                                        const int64_t* rng, int64_t rows, int64_t cols, void* dx, int64_t lddx,
+                                        void* dresidual, int64_t lddr, void* dweight, void* dbias, void* workspace,
+                                        size_t workspace_bytes, otf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Gated feed-forward block: y = (act(x w_gate^T) * (x w_up^T)) w_down^T, and its backward
+ * pass.  x, y: (rows, d); w_gate, w_up: (f, d); w_down: (d, f); all of one dtype, float32
+ * accumulation.  Weights' leading dimension: at most 2^20, d and f too.
+ *
+ * saved: what backward needs of the forward call (the gate and up products and h), opaque,
+ *   otf_gated_ffn_saved_size bytes, 16-byte aligned; NULL in inference.  workspace: 16-byte
+ *   aligned, at least ..._workspace_size bytes of the SAME arguments (pointers included: an
+ *   operand whose rows are not 16-byte aligned is copied to one whose are); it may be reused
+ *   as soon as the call's work on the stream is done.
+ * Backward reads dy, x, the weights and saved.  dx NULL: not computed; dw_gate and dw_up go
+ *   together (one leading dimension), dw_down by itself.
+ * rows = 0: forward does nothing, backward zeroes the weight gradients.                      */
+typedef enum { OTF_ACT_SILU = 0, OTF_ACT_GELU = 1 } otf_activation;   /* gelu: the exact form, by erf */
+typedef struct {
+    int64_t rows, d, f;
+    int32_t dtype, activation;
+    const void* x;       int64_t ldx;
+    const void* w_gate;
+    const void* w_up;    int64_t ldw_in;
+    const void* w_down;  int64_t ldw_down;
+    void* y;             int64_t ldy;
+    void* saved;
+    const void* dy;      int64_t lddy;
+    void* dx;            int64_t lddx;
+    void* dw_gate;
+    void* dw_up;         int64_t lddw_in;
+    void* dw_down;       int64_t lddw_down;
+} otf_ffn_args;
+size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype);
+size_t otf_gated_ffn_workspace_size(const otf_ffn_args* args);
+int otf_gated_ffn(const otf_ffn_args* args, void* workspace, size_t workspace_bytes, otf_stream_t stream);
+size_t otf_gated_ffn_backward_workspace_size(const otf_ffn_args* args);
+int otf_gated_ffn_backward(const otf_ffn_args* args, void* workspace, size_t workspace_bytes, otf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

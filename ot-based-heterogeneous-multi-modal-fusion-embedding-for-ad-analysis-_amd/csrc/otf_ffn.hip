@@ -1,0 +1,813 @@
+// otf_ffn.hip — the gated feed-forward block, forward and backward, on the matrix cores.
+//
+//   forward    h = act(x Wg^T) * (x Wu^T)        one kernel: both products share x, gate and up
+//              y = h Wd^T                        of a feature meet in one lane's registers
+//   backward   dh = dy Wd;  dg = dh u act'(g), du = dh act(g)    epilogue of the dh product
+//              dx = dg Wg + du Wu                one product over 2 f, two segments of K
+//              dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// Every product is C[m, n] = sum_k A(m, k) B(n, k) with each operand either K-contiguous
+// (layout K: rows are m or n) or row-contiguous (layout T: rows are k).  Both go global -> LDS
+// by 16-byte buffer loads that write LDS directly; what lies past an operand's end comes back
+// as zero from the buffer descriptor's range check, so ragged edges cost no branch.  Layout T
+// is transposed on the way from LDS to registers (ds_read_b64_tr_b16).
+//
+// All sums are float32 in the accumulators.  h, and g and u for the backward pass, are kept in
+// the operands' type: one rounding each, which the products that read them need anyway.
+#include "otf_rng.h"
+
+namespace otf {
+namespace {
+
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 b16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
+
+[[maybe_unused]] constexpr int kRsrcFlags = 0x00020000;   // raw buffer of 32-bit data
+constexpr int kTileBytes = 128;          // depth of a K-tile: 64 16-bit or 32 float32 values
+
+// ---- one 16 x 16 block over 64 bytes of K ---------------------------------------------
+// A fragment is 16 bytes a lane: row lane % 16, K chunk lane / 16.  For float32 the four
+// values feed four 16x16x4 steps; both operands name the same k for a lane and step, which is
+// all the sum needs.
+template <typename T> struct Frag;
+template <> struct Frag<_Float16> {
+    using type = f16x8;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Frag<__bf16> {
+    using type = b16x8;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Frag<float> {
+    using type = f32x4;
+    static __device__ __forceinline__ f32x4 mma(type a, type b, f32x4 c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ---- activations ------------------------------------------------------------------------
+enum { kSilu = 0, kGelu = 1 };
+__device__ __forceinline__ float act_value(int act, float g) {
+    if (act == kSilu) return g / (1.0f + expf(-g));
+    return 0.5f * g * erfcf(-0.70710678118654752f * g);
+}
+__device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
+    if (act == kSilu) {
+        const float s = 1.0f / (1.0f + expf(-g));
+        a = g * s;
+        da = s * (1.0f + g * (1.0f - s));
+    } else {
+        const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+        a = g * c;
+        da = c + g * 0.39894228040143268f * expf(-0.5f * g * g);
+    }
+}
+
+// ---- operands -----------------------------------------------------------------------------
+// One tile of R rows (m or n) by a K-tile, R * 128 bytes of LDS.
+//   layout K: two halves of 64 bytes of K, each [R][64 B], the four 16-byte chunks of a row
+//             permuted by the row, so 16 rows' fragments of one chunk fall on different banks
+//   layout T: [k][R values], the 16-byte chunks of a row permuted by k so that the rows that
+//             one LDS read spans fall on different banks
+struct Operand {
+    const char* p[2];   // second segment of K, or the second half of the tile (gated)
+    int64_t ld;         // bytes
+    int mn;             // valid rows (K) / columns (T)
+    int k;              // valid k
+};
+
+__device__ __forceinline__ int swz_k(int row) { return (0x78 >> (2 * ((row >> 2) & 3))) & 3; }
+template <typename T, int R> __device__ __forceinline__ int swz_t(int k) {
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (R >= 128) return 2 * ((k & 3) | (((k >> 3) & 1) << 2));
+        if constexpr (R == 64) return 2 * (((k >> 1) & 1) | (((k >> 3) & 1) << 1));
+        if constexpr (R == 32) return 2 * ((k >> 3) & 1);
+        return 0;
+    } else {
+        if constexpr (R >= 64) return 4 * ((k >> 2) & 3);
+        if constexpr (R == 32) return 4 * ((k >> 2) & 1);
+        return 0;
+    }
+}
+
+template <typename T, bool TR, int R, int NT> struct Tile {
+    static constexpr int BYTES = R * kTileBytes, CHUNKS = BYTES / 16, PER = (CHUNKS + NT - 1) / NT;
+    static constexpr int BK = kTileBytes / (int)sizeof(T);
+    static constexpr int CPR = R * (int)sizeof(T) / 16;   // layout T: chunks of a k row
+    uint32_t off[PER];
+    int kb[PER];   // layout K: byte of K of the lane's chunk
+
+    __device__ __forceinline__ void init(int64_t ld) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = i * NT + (int)threadIdx.x;
+            if constexpr (TR) {
+                const int k = c / CPR, chunk = (c % CPR) ^ swz_t<T, R>(k);
+                off[i] = (uint32_t)(k * ld) + chunk * 16;
+                kb[i] = 0;
+            } else {
+                const int half = c / (R * 4), row = (c % (R * 4)) >> 2, chunk = (c & 3) ^ swz_k(row);
+                kb[i] = half * 64 + chunk * 16;
+                off[i] = (uint32_t)(row * ld) + kb[i];
+            }
+        }
+    }
+    // K-tile kt of the operand whose first row (K) / column (T) is at `base`, of which `mn`
+    // remain, into LDS at `dst`
+    __device__ __forceinline__ void stage(const char* base, int64_t ld, int mn, int kvalid, int kt, char* dst) const {
+#ifdef __HIP_DEVICE_COMPILE__   // the buffer builtins: the host pass drops the launch stubs of kernels that reach them
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if constexpr (TR) {
+            const int rows = min(kvalid - kt * BK, BK);
+            const int64_t bytes = rows > 0 && mn > 0 ? (rows - 1) * ld + (int64_t)min(mn, R) * (int)sizeof(T) : 0;
+            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)kt * BK * ld), 0, (int)bytes, kRsrcFlags);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if ((i + 1) * NT <= CHUNKS || i * NT + wave * 64 < CHUNKS)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16, off[i], 0, 0, 0);
+        } else {
+            const int left = kvalid * (int)sizeof(T) - kt * kTileBytes;   // bytes of K still ahead
+            const int64_t bytes = mn > 0 && left > 0 ? (int64_t)(min(mn, R) - 1) * ld + left : 0;
+            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)kt * kTileBytes), 0, (int)bytes, kRsrcFlags);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                if ((i + 1) * NT <= CHUNKS || i * NT + wave * 64 < CHUNKS)
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                        r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16,
+                        kb[i] < left ? off[i] : 0xfffffff0u, 0, 0, 0);
+        }
+#endif
+    }
+    // fragment of the 16 rows from r0, K half s
+    static __device__ __forceinline__ typename Frag<T>::type frag(const char* tile, int r0, int s, int lane) {
+        if constexpr (!TR) {
+            const int row = r0 + (lane & 15);
+            return *reinterpret_cast<const typename Frag<T>::type*>(tile + s * (R * 64) + row * 64 +
+                                                                    (((lane >> 4) ^ swz_k(row)) << 4));
+        } else if constexpr (sizeof(T) == 2) {
+            const int i = lane & 15, k = s * 32 + (lane >> 4) * 8 + (i >> 2), chunk = r0 / 8 + ((i & 3) >> 1);
+            const char* a = tile + k * (R * 2) + (i & 1) * 8;
+            typename Frag<T>::type f;
+            s16x4* h = reinterpret_cast<s16x4*>(&f);
+            h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(a + ((chunk ^ swz_t<T, R>(k)) << 4)));
+            h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(a + 4 * (R * 2) + ((chunk ^ swz_t<T, R>(k + 4)) << 4)));
+            return f;
+        } else {
+            typename Frag<T>::type f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int k = s * 16 + (lane >> 4) * 4 + j, c = r0 + (lane & 15);
+                f[j] = *reinterpret_cast<const float*>(tile + k * (R * 4) + (((c >> 2) ^ swz_t<T, R>(k)) << 4) + (c & 3) * 4);
+            }
+            return f;
+        }
+    }
+};
+
+// ---- results ------------------------------------------------------------------------------
+enum { kStore = 0, kPartial = 1, kGatedForward = 2, kGatedBackward = 3 };
+struct GemmArgs {
+    Operand a, b;
+    int M, N;            // extent of the result; gated forward: N = features
+    int segments;        // of K (each a.k deep)
+    int splits;          // of the K-tiles, kPartial: one slab of C each
+    int tiles_m, tiles_n;
+    void* c[2];          // result; second: the rows past tiles of the first (batch), see batch
+    int64_t ldc;         // elements
+    int batch;           // 2: a.p[1] -> c[1] as a second product of the same shape
+    int act;
+    const void* g;       // gated: saved gate and up products (backward: in; forward: out or null)
+    const void* u;
+    void* h;             // gated forward: h; backward: dg
+    void* h2;            // gated backward: du
+    int64_t ldh;         // elements, of g, u, h, h2
+};
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int valid, bool vec, f32x4 v) {
+    if (vec && valid >= 4) {
+        using V = T __attribute__((ext_vector_type(4)));
+        V q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[j] = (T)v[j];
+        *reinterpret_cast<V*>(p) = q;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < valid) p[j] = (T)v[j];
+    }
+}
+template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
+    using V = T __attribute__((ext_vector_type(4)));
+    const V q = *reinterpret_cast<const V*>(p);
+    return f32x4{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
+}
+
+// four consecutive columns n.. of row m: acc0 of the tile's first half, acc1 of its second
+// (at n2; gated forward: the up product of the same columns)
+template <typename T, int EPI>
+__device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int m, int n, int n2, f32x4 acc0, f32x4 acc1) {
+    if (m >= a.M) return;
+    if constexpr (EPI == kStore) {
+        T* c = (T*)a.c[z] + (int64_t)m * a.ldc;
+        const bool vec = (a.ldc & 3) == 0 && ((uintptr_t)a.c[z] & (4 * sizeof(T) - 1)) == 0;
+        store4(c + n, a.N - n, vec, acc0);
+        store4(c + n2, a.N - n2, vec, acc1);
+    } else if constexpr (EPI == kPartial) {   // ldc: a multiple of 4 past N
+        float* c = (float*)a.c[0] + (((int64_t)split * a.batch + z) * a.M + m) * a.ldc;
+        if (n < a.N) *reinterpret_cast<f32x4*>(c + n) = acc0;
+        if (n2 < a.N) *reinterpret_cast<f32x4*>(c + n2) = acc1;
+    } else if constexpr (EPI == kGatedForward) {
+        if (n >= a.N) return;   // N, ldh multiples of 8
+        const int64_t o = (int64_t)m * a.ldh + n;
+        f32x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = act_value(a.act, acc0[j]) * acc1[j];
+        store4((T*)a.h + o, 4, true, h);
+        if (a.g) {
+            store4((T*)const_cast<void*>(a.g) + o, 4, true, acc0);
+            store4((T*)const_cast<void*>(a.u) + o, 4, true, acc1);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int nn = i ? n2 : n;
+            if (nn >= a.N) continue;
+            const int64_t o = (int64_t)m * a.ldh + nn;
+            const f32x4 g = load4((const T*)a.g + o), u = load4((const T*)a.u + o), dh = i ? acc1 : acc0;
+            f32x4 dg, du;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float v, dv;
+                act_both(a.act, g[j], v, dv);
+                dg[j] = dh[j] * u[j] * dv;
+                du[j] = dh[j] * v;
+            }
+            store4((T*)a.h + o, 4, true, dg);
+            store4((T*)a.h2 + o, 4, true, du);
+        }
+    }
+}
+
+// Workgroup -> tile.  Consecutive ids go to the 8 XCDs in turn; each XCD gets a run of
+// consecutive tiles, walked in groups of 8 row tiles, so its L2 holds the operands they share.
+__device__ __forceinline__ void tile_of(int id, int count, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int q = count / 8, r = count % 8, x = id % 8;
+    const int t = (x < r ? x * (q + 1) : r * (q + 1) + (x - r) * q) + id / 8;
+    const int per = 8 * tiles_n, g = t / per, first = g * 8, rows = min(tiles_m - first, 8), in = t - g * per;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+// ---- the tiled product -----------------------------------------------------------------
+// TM x TN tile (B in two halves of TN / 2), WGM x WGN waves; K-tiles double-buffered: the
+// next one is on its way while this one's MFMAs run, one barrier a K-tile.
+template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int EPI>
+__global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
+    constexpr int NT = 64 * WGM * WGN, TH = TN / 2, RA = TM / WGM / 16, RB = TH / WGN / 16;
+    using TA = Tile<T, TRA, TM, NT>;
+    using TB = Tile<T, TRB, TH, NT>;
+    constexpr int BUF = TA::BYTES + 2 * TB::BYTES;
+    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / WGN, wn = wid % WGN;
+
+    const int tiles = a.tiles_m * a.tiles_n, z = blockIdx.y % a.batch, split = blockIdx.y / a.batch;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles, a.tiles_m, a.tiles_n, tm, tn);
+    const int m0 = tm * TM, n0 = EPI == kGatedForward ? tn * TH : tn * TN;
+
+    TA ta;
+    TB tb;
+    ta.init(a.a.ld);
+    tb.init(a.b.ld);
+    const int64_t am = TRA ? (int64_t)m0 * (int)sizeof(T) : (int64_t)m0 * a.a.ld;
+    const int64_t bn = TRB ? (int64_t)n0 * (int)sizeof(T) : (int64_t)n0 * a.b.ld;
+    const int64_t bh = TRB ? (int64_t)TH * (int)sizeof(T) : (int64_t)TH * a.b.ld;
+
+    const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
+    const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
+    auto stage = [&](int kt, int buf) {
+        const int seg = kt >= nk ? 1 : 0, k = kt - seg * nk;
+        char* dst = smem + buf * BUF;
+        ta.stage(a.a.p[a.batch > 1 ? z : seg] + am, a.a.ld, a.a.mn - m0, a.a.k, k, dst);
+        const char* b0 = a.b.p[EPI == kGatedForward ? 0 : seg] + bn;
+        const char* b1 = EPI == kGatedForward ? a.b.p[1] + bn : b0 + bh;
+        tb.stage(b0, a.b.ld, a.b.mn - n0, a.b.k, k, dst + TA::BYTES);
+        tb.stage(b1, a.b.ld, EPI == kGatedForward ? a.b.mn - n0 : a.b.mn - n0 - TH, a.b.k, k, dst + TA::BYTES + TB::BYTES);
+    };
+
+    f32x4 acc[2][RB][RA];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < RB; ++j)
+#pragma unroll
+            for (int i = 0; i < RA; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (k0 < k1) stage(k0, 0);
+    for (int kt = k0; kt < k1; ++kt) {
+        const int buf = (kt - k0) & 1;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        // every fragment of the K-tile first, then the next tile's loads: the compiler waits
+        // for loads in flight before a transposed LDS read, so none may be
+        const char* sa = smem + buf * BUF;
+        const char* sb = sa + TA::BYTES;
+        typename Frag<T>::type fa[2][RA], fb[2][2][RB];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int i = 0; i < RA; ++i) fa[s][i] = TA::frag(sa, (wm * RA + i) * 16, s, lane);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < RB; ++j) fb[s][h][j] = TB::frag(sb + h * TB::BYTES, (wn * RB + j) * 16, s, lane);
+        }
+        asm volatile("" ::: "memory");
+        if (kt + 1 < k1) stage(kt + 1, buf ^ 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < RB; ++j)
+#pragma unroll
+                    for (int i = 0; i < RA; ++i) acc[h][j][i] = Frag<T>::mma(fb[s][h][j], fa[s][i], acc[h][j][i]);
+    }
+    // B is the first operand of the MFMAs, so a lane holds four consecutive n of one m
+#pragma unroll
+    for (int i = 0; i < RA; ++i)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) {
+            const int m = m0 + (wm * RA + i) * 16 + (lane & 15), n = n0 + (wn * RB + j) * 16 + (lane >> 4) * 4;
+            finish4<T, EPI>(a, z, split, m, n, n + TH, acc[0][j][i], acc[1][j][i]);
+        }
+}
+
+// slabs [splits][batch][M][ldp] added in order and rounded once
+template <typename T>
+__global__ __launch_bounds__(256) void ffn_join_kernel(const float* __restrict__ slab, int splits, int batch, int64_t M,
+                                                       int N, int64_t ldp, T* c0, T* c1, int64_t ldc) {
+    const int64_t per = ldp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= M * batch * per) return;
+    const int64_t zm = i / per, n = (i - zm * per) * 4, z = zm / M, m = zm - z * M;
+    if (n >= N) return;
+    f32x4 s = *reinterpret_cast<const f32x4*>(slab + zm * ldp + n);
+    for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(slab + ((int64_t)k * batch * M + zm) * ldp + n);
+    T* c = (z ? c1 : c0) + m * ldc;
+    const bool vec = (ldc & 3) == 0 && ((uintptr_t)(z ? c1 : c0) & (4 * sizeof(T) - 1)) == 0;
+    store4(c + n, (int)(N - n < 4 ? N - n : 4), vec, s);
+}
+
+// ---- few rows ------------------------------------------------------------------------------
+// Up to 16 rows of x: the weights are read once, straight into registers, and bound the time.
+// A workgroup takes 16 features (GATED: of both weights); its NW waves take 128-byte pieces of
+// K in turn and meet in LDS.  Rows of x past the last are zero fragments.
+template <typename T, bool GATED, int NW>
+__global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ x, int64_t ldx, int rows,
+                                                          const T* __restrict__ w0, const T* __restrict__ w1,
+                                                          int64_t ldw, int K, int N, int act, T* __restrict__ out,
+                                                          int64_t ldo, T* __restrict__ sg, T* __restrict__ su) {
+    constexpr int NB = GATED ? 2 : 1, PIECE = 128 / (int)sizeof(T), CH = 16 / (int)sizeof(T);
+    constexpr int UNROLL = GATED ? 2 : 4;
+    __shared__ f32x4 part[NW][NB][64];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, r = lane & 15, kc = lane >> 4;
+    const int n0 = blockIdx.x * 16;
+    const int64_t wrow = n0 + r < N ? n0 + r : N - 1;   // past the end: read the last row, drop the result
+    const T* pw[2] = {w0 + wrow * ldw, GATED ? w1 + wrow * ldw : nullptr};
+    const T* px = x + (int64_t)(r < rows ? r : 0) * ldx;
+    const bool live = r < rows;
+    using F = typename Frag<T>::type;
+    using U = T __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    auto chunk = [&](const T* p, int k) -> F {
+        F f{};
+        if (k + CH <= K) {
+            const U q = *reinterpret_cast<const U*>(p + k);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) f[j] = q[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+                if (k + j < K) f[j] = p[k + j];
+        }
+        return f;
+    };
+    f32x4 acc[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = wid * PIECE; k0 < K; k0 += NW * PIECE * UNROLL) {
+        F fw[UNROLL][2][NB], fx[UNROLL][2];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int k = k0 + u * NW * PIECE + (s * 4 + kc) * CH;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) fw[u][s][b] = chunk(pw[b], k);
+                fx[u][s] = live ? chunk(px, k) : F{};
+            }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[b] = Frag<T>::mma(fw[u][s][b], fx[u][s], acc[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) part[wid][b][lane] = acc[b];
+    __syncthreads();
+    if (wid) return;
+    f32x4 s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        s[b] = part[0][b][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) s[b] += part[w][b][lane];
+    }
+    if (!live) return;
+    const int n = n0 + kc * 4;
+    if constexpr (GATED) {   // ldo a multiple of 8, columns up to it written (zeros past N)
+        f32x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (n + j >= N) s[0][j] = s[1][j] = 0.0f;
+            h[j] = act_value(act, s[0][j]) * s[1][j];
+        }
+        if (n >= ldo) return;
+        const int64_t o = (int64_t)r * ldo + n;
+        store4(out + o, 4, true, h);
+        if (sg) {
+            store4(sg + o, 4, true, s[0]);
+            store4(su + o, 4, true, s[1]);
+        }
+    } else {
+        const bool vec = (ldo & 3) == 0 && ((uintptr_t)out & (4 * sizeof(T) - 1)) == 0;
+        store4(out + (int64_t)r * ldo + n, N - n, vec, s[0]);
+    }
+}
+
+// ---- copies for unaligned operands ---------------------------------------------------------
+// Rows copied to a leading dimension that is a multiple of 8, zeros past the last column.
+struct PackItem {
+    const void* src;
+    void* dst;
+    int64_t lds, ldd, rows, cols, first;   // first: index of the item's first chunk of 8
+};
+struct PackArgs {
+    PackItem item[5];
+    int count;
+    int64_t total;
+};
+template <typename T> __global__ __launch_bounds__(256) void ffn_pack_kernel(PackArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.total) return;
+    int k = 0;
+    while (k + 1 < a.count && i >= a.item[k + 1].first) ++k;
+    const PackItem& it = a.item[k];
+    const int64_t per = it.ldd / 8, j = i - it.first, row = j / per, col = (j - row * per) * 8;
+    float v[8];
+    const int64_t left = it.cols - col;
+    load8((const T*)it.src + row * it.lds + col, (int)(left < 8 ? left : 8), v);
+    store8((T*)it.dst + row * it.ldd + col, 8, v);
+}
+template <typename T> __global__ __launch_bounds__(256) void ffn_zero_kernel(T* p, int64_t rows, int64_t cols, int64_t ld) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < rows * cols) p[i / cols * ld + i % cols] = (T)0.0f;
+}
+
+// ------------------------------------------------------------------------------------- host
+int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+size_t esize(int32_t t) { return t == OTF_F32 ? 4 : 2; }
+
+struct Carver {
+    char* base;
+    size_t used = 0;
+    void* take(size_t bytes) {
+        void* p = base ? base + used : nullptr;
+        used += up256(bytes);
+        return p;
+    }
+};
+
+// A product: operand layouts, extents, and what becomes of the result
+struct Product {
+    bool tra, trb;
+    int epi;
+    GemmArgs a;
+};
+
+constexpr int kCus = 256;   // MI355X; only tile choice depends on it
+
+// Tile 128 x 128 where that fills the chip, else 64 x 64; K split into slabs where even the
+// small tiles leave most of it idle.
+struct Plan {
+    int tm, tn, splits;
+};
+Plan plan_product(const Product& p, int elem) {
+    const GemmArgs& a = p.a;
+    auto tiles = [&](int t) {
+        const int64_t m = (a.M + t - 1) / t, n = p.epi == kGatedForward ? (2 * (int64_t)a.N + t - 1) / t : (a.N + t - 1) / t;
+        return m * n * a.batch;
+    };
+    const int side = tiles(128) >= kCus ? 128 : 64;
+    int splits = 1;
+    if (p.epi == kStore) {
+        const int64_t ktiles = (int64_t)(a.a.k + kTileBytes / elem - 1) / (kTileBytes / elem) * a.segments, t = tiles(side);
+        while (t * splits * 2 <= 2 * kCus && ktiles / (splits * 2) >= 4) splits *= 2;
+    }
+    return Plan{side, side, splits};
+}
+size_t slab_bytes(const Product& p, const Plan& q) {
+    return q.splits > 1 ? (size_t)q.splits * p.a.batch * p.a.M * (size_t)up8(p.a.N) * 4 : 0;
+}
+
+template <typename T, bool TRA, bool TRB, int EPI>
+hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
+    a.splits = q.splits;
+    a.tiles_m = (a.M + q.tm - 1) / q.tm;
+    const int cols = EPI == kGatedForward ? q.tn / 2 : q.tn;
+    a.tiles_n = (a.N + cols - 1) / cols;
+    const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
+    if (q.tm == 128)
+        ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
+    else
+        ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename T, bool TRA, bool TRB>
+hipError_t run_store(const Product& p, float* slab, hipStream_t s) {
+    const Plan q = plan_product(p, (int)sizeof(T));
+    if (q.splits == 1) return launch_tiles<T, TRA, TRB, kStore>(p.a, q, s);
+    GemmArgs a = p.a;
+    a.c[0] = slab;
+    a.ldc = up8(a.N);
+    const hipError_t e = launch_tiles<T, TRA, TRB, kPartial>(a, q, s);
+    if (e != hipSuccess) return e;
+    const int64_t work = (int64_t)a.M * a.batch * (a.ldc / 4);
+    ffn_join_kernel<T><<<(unsigned)((work + 255) / 256), 256, 0, s>>>(slab, q.splits, a.batch, a.M, a.N, a.ldc,
+                                                                     (T*)p.a.c[0], (T*)p.a.c[1], p.a.ldc);
+    return hipGetLastError();
+}
+
+// The block's buffers and products.  Built twice: for the sizes (null pointers) and to run.
+struct Block {
+    const otf_ffn_args* o;
+    int es;
+    int64_t n, d, f, d8, f8;
+    Operand x{}, wg{}, wu{}, wd{}, dy{};
+    PackArgs pack{};
+    Carver ws;
+
+    static bool aligned(const void* p, int64_t ld, int64_t cols) {
+        return cols % 8 == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
+    }
+    void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols, bool copy) {
+        v.p[0] = v.p[1] = (const char*)p;
+        v.ld = ld * es;
+        if (copy) {
+            const int64_t ldd = up8(cols);
+            void* dst = ws.take((size_t)(rows * ldd * es));
+            pack.item[pack.count++] = PackItem{p, dst, ld, ldd, rows, cols, pack.total};
+            pack.total += rows * (ldd / 8);
+            v.p[0] = v.p[1] = (const char*)dst;
+            v.ld = ldd * es;
+        }
+    }
+    void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols) {
+        operand(v, p, ld, rows, cols, !aligned(p, ld, cols));
+    }
+    // gate and up: one leading dimension, so both are copied or none
+    void weights_in() {
+        const bool copy = !aligned(o->w_gate, o->ldw_in, d) || !aligned(o->w_up, o->ldw_in, d);
+        operand(wg, o->w_gate, o->ldw_in, f, d, copy);
+        operand(wu, o->w_up, o->ldw_in, f, d, copy);
+    }
+    template <typename T> hipError_t run_pack(hipStream_t s) {
+        if (!pack.count) return hipSuccess;
+        ffn_pack_kernel<T><<<(unsigned)((pack.total + 255) / 256), 256, 0, s>>>(pack);
+        return hipGetLastError();
+    }
+};
+
+Operand as_operand(const Operand& v, int64_t mn, int64_t k) {
+    Operand r = v;
+    r.mn = (int)mn;
+    r.k = (int)k;
+    return r;
+}
+Operand buffer_operand(const void* p, int64_t ld, int es, int64_t mn, int64_t k) {
+    return Operand{{(const char*)p, (const char*)p}, ld * es, (int)mn, (int)k};
+}
+GemmArgs product_args(const Operand& a, const Operand& b, int64_t M, int64_t N, void* c, int64_t ldc) {
+    GemmArgs g{};
+    g.a = a, g.b = b, g.M = (int)M, g.N = (int)N, g.segments = 1, g.splits = 1, g.batch = 1;
+    g.c[0] = c, g.ldc = ldc;
+    return g;
+}
+
+constexpr int kFewRows = 16;   // one MFMA tile of rows
+
+int check_ffn(const otf_ffn_args* o) {
+    if (!o) return OTF_EINVAL;
+    if (o->dtype != OTF_F32 && o->dtype != OTF_F16 && o->dtype != OTF_BF16) return OTF_EINVAL;
+    if (o->activation != OTF_ACT_SILU && o->activation != OTF_ACT_GELU) return OTF_EINVAL;
+    if (o->rows < 0 || o->d <= 0 || o->f <= 0) return OTF_EINVAL;
+    // 32-bit element counts of a row tile and of the K extents
+    if (o->rows > INT32_MAX / 8 || o->d > (1 << 20) || o->f > (1 << 20)) return OTF_EUNSUPPORTED;
+    return OTF_OK;
+}
+// leading dimensions: 256 rows within a 31-bit byte offset
+bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > (1 << 20); }
+bool misaligned(const void* p, int32_t dtype) { return (uintptr_t)p % esize(dtype) != 0; }
+
+struct Saved {
+    char *g, *u, *h;
+};
+Saved carve_saved(void* p, int64_t n, int64_t f8, int es) {
+    const size_t one = up256((size_t)(n * f8 * es));
+    char* b = (char*)p;
+    return Saved{b, b + one, b + 2 * one};
+}
+
+// forward: returns the workspace it needs in *need; runs where run is set
+template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
+    Block b{};
+    b.o = o, b.es = (int)sizeof(T), b.n = o->rows, b.d = o->d, b.f = o->f, b.d8 = up8(o->d), b.f8 = up8(o->f);
+    b.ws.base = (char*)workspace;
+    const bool few = b.n <= kFewRows;
+    Saved sv{};
+    if (o->saved)
+        sv = carve_saved(o->saved, b.n, b.f8, b.es);
+    else
+        sv.h = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
+    if (few) {
+        *need = b.ws.used;
+        if (!run) return OTF_OK;
+        const unsigned g1 = (unsigned)((b.f8 + 15) / 16), g2 = (unsigned)((b.d + 15) / 16);
+        ffn_few_kernel<T, true, 4><<<g1, 256, 0, s>>>((const T*)o->x, o->ldx, (int)b.n, (const T*)o->w_gate,
+                                                       (const T*)o->w_up, o->ldw_in, (int)b.d, (int)b.f, o->activation,
+                                                       (T*)sv.h, b.f8, (T*)sv.g, (T*)sv.u);
+        OTF_HIP(hipGetLastError());
+        ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.f8, (int)b.n, (const T*)o->w_down, nullptr,
+                                                        o->ldw_down, (int)b.f, (int)b.d, 0, (T*)o->y, o->ldy, nullptr,
+                                                        nullptr);
+        return check_hip(hipGetLastError());
+    }
+    b.operand(b.x, o->x, o->ldx, b.n, b.d);
+    b.weights_in();
+    b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
+    Product in{false, false, kGatedForward, product_args(as_operand(b.x, b.n, b.d8), as_operand(b.wg, b.f, b.d8), b.n, b.f8, nullptr, 0)};
+    in.a.b.p[1] = b.wu.p[0];
+    in.a.act = o->activation, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.f8;
+    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.f8, b.es, b.n, b.f8), as_operand(b.wd, b.d, b.f8), b.n, b.d, o->y, o->ldy)};
+    float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es)));
+    *need = b.ws.used;
+    if (!run) return OTF_OK;
+    OTF_HIP(b.run_pack<T>(s));
+    OTF_HIP((launch_tiles<T, false, false, kGatedForward>(in.a, plan_product(in, b.es), s)));
+    OTF_HIP((run_store<T, false, false>(down, slab, s)));
+    return OTF_OK;
+}
+
+template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
+    Block b{};
+    b.o = o, b.es = (int)sizeof(T), b.n = o->rows, b.d = o->d, b.f = o->f, b.d8 = up8(o->d), b.f8 = up8(o->f);
+    b.ws.base = (char*)workspace;
+    const Saved sv = carve_saved(o->saved, b.n, b.f8, b.es);
+    const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
+    char* dg = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
+    char* du = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
+    b.operand(b.dy, o->dy, o->lddy, b.n, b.d);
+    if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
+    if (wx) b.weights_in();
+    if (win) b.operand(b.x, o->x, o->ldx, b.n, b.d);
+    // dh = dy Wd: K = d; Wd's rows are k
+    Product mid{false, true, kGatedBackward, product_args(as_operand(b.dy, b.n, b.d8), as_operand(b.wd, b.f8, b.d), b.n, b.f8, nullptr, 0)};
+    mid.a.act = o->activation, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.f8;
+    // dx = dg Wg + du Wu: two segments of K = f
+    Product px{false, true, kStore, product_args(buffer_operand(dg, b.f8, b.es, b.n, b.f8), as_operand(b.wg, b.d8, b.f), b.n, b.d, o->dx, o->lddx)};
+    px.a.a.p[1] = du, px.a.b.p[1] = b.wu.p[0], px.a.segments = 2;
+    // dWg, dWu = dg^T x, du^T x: a batch of two, K = rows
+    Product pi{true, true, kStore, product_args(buffer_operand(dg, b.f8, b.es, b.f8, b.n), as_operand(b.x, b.d8, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
+    pi.a.a.p[1] = du, pi.a.c[1] = o->dw_up, pi.a.batch = 2;
+    // dWd = dy^T h
+    Product pd{true, true, kStore, product_args(as_operand(b.dy, b.d8, b.n), buffer_operand(sv.h, b.f8, b.es, b.f8, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
+    size_t slab = 0;   // one after another on the stream: they share it
+    auto more = [&](const Product& p) { const size_t k = slab_bytes(p, plan_product(p, b.es)); slab = k > slab ? k : slab; };
+    if (wx) more(px);
+    if (win) more(pi);
+    if (wdown) more(pd);
+    float* part = (float*)b.ws.take(slab);
+    *need = b.ws.used;
+    if (!run) return OTF_OK;
+    OTF_HIP(b.run_pack<T>(s));
+    if (wx || win) OTF_HIP((launch_tiles<T, false, true, kGatedBackward>(mid.a, plan_product(mid, b.es), s)));
+    if (wx) OTF_HIP((run_store<T, false, true>(px, part, s)));
+    if (win) OTF_HIP((run_store<T, true, true>(pi, part, s)));
+    if (wdown) OTF_HIP((run_store<T, true, true>(pd, part, s)));
+    return OTF_OK;
+}
+
+template <typename T> hipError_t zero_rows(void* p, int64_t rows, int64_t cols, int64_t ld, hipStream_t s) {
+    ffn_zero_kernel<T><<<(unsigned)((rows * cols + 255) / 256), 256, 0, s>>>((T*)p, rows, cols, ld);
+    return hipGetLastError();
+}
+
+int forward_any(const otf_ffn_args* o, void* ws, size_t* need, bool run, hipStream_t s) {
+    if (o->dtype == OTF_F32) return forward<float>(o, ws, need, run, s);
+    if (o->dtype == OTF_F16) return forward<_Float16>(o, ws, need, run, s);
+    return forward<__bf16>(o, ws, need, run, s);
+}
+int backward_any(const otf_ffn_args* o, void* ws, size_t* need, bool run, hipStream_t s) {
+    if (o->dtype == OTF_F32) return backward<float>(o, ws, need, run, s);
+    if (o->dtype == OTF_F16) return backward<_Float16>(o, ws, need, run, s);
+    return backward<__bf16>(o, ws, need, run, s);
+}
+
+}  // namespace
+}  // namespace otf
+
+using namespace otf;
+
+extern "C" {
+
+size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype) {
+    if (rows <= 0 || f <= 0) return 0;
+    return 3 * up256((size_t)(rows * up8(f)) * esize(dtype));
+}
+
+size_t otf_gated_ffn_workspace_size(const otf_ffn_args* o) {
+    size_t need = 0;
+    if (check_ffn(o) != OTF_OK || o->rows == 0) return 0;
+    forward_any(o, nullptr, &need, false, nullptr);
+    return need;
+}
+
+size_t otf_gated_ffn_backward_workspace_size(const otf_ffn_args* o) {
+    size_t need = 0;
+    if (check_ffn(o) != OTF_OK || o->rows == 0) return 0;
+    backward_any(o, nullptr, &need, false, nullptr);
+    return need;
+}
+
+int otf_gated_ffn(const otf_ffn_args* o, void* workspace, size_t workspace_bytes, otf_stream_t stream) {
+    const int rc = check_ffn(o);
+    if (rc != OTF_OK || o->rows == 0) return rc;
+    if (!o->x || !o->w_gate || !o->w_up || !o->w_down || !o->y) return OTF_EINVAL;
+    if (bad_ld(o->ldx, o->d) || bad_ld(o->ldw_in, o->d) || bad_ld(o->ldw_down, o->f) || o->ldy < o->d) return OTF_EINVAL;
+    for (const void* p : {o->x, o->w_gate, o->w_up, o->w_down, (const void*)o->y})
+        if (misaligned(p, o->dtype)) return OTF_EINVAL;
+    if ((uintptr_t)o->saved % 16 || (uintptr_t)workspace % 16) return OTF_EINVAL;
+    size_t need = 0;
+    const int rs = forward_any(o, nullptr, &need, false, nullptr);
+    if (rs != OTF_OK) return rs;
+    if (need && (!workspace || workspace_bytes < need)) return OTF_EINVAL;
+    return forward_any(o, workspace, &need, true, (hipStream_t)stream);
+}
+
+int otf_gated_ffn_backward(const otf_ffn_args* o, void* workspace, size_t workspace_bytes, otf_stream_t stream) {
+    const int rc = check_ffn(o);
+    if (rc != OTF_OK) return rc;
+    if ((o->dw_gate == nullptr) != (o->dw_up == nullptr)) return OTF_EINVAL;
+    hipStream_t s = (hipStream_t)stream;
+    if (o->dw_gate && (o->lddw_in < o->d || misaligned(o->dw_gate, o->dtype) || misaligned(o->dw_up, o->dtype))) return OTF_EINVAL;
+    if (o->dw_down && (o->lddw_down < o->f || misaligned(o->dw_down, o->dtype))) return OTF_EINVAL;
+    if (o->rows == 0) {   // no row: the sums are zero
+        auto zero = [&](void* p, int64_t r, int64_t c, int64_t ld) {
+            if (!p) return hipSuccess;
+            return o->dtype == OTF_F32 ? zero_rows<float>(p, r, c, ld, s) : zero_rows<_Float16>(p, r, c, ld, s);
+        };
+        OTF_HIP(zero(o->dw_gate, o->f, o->d, o->lddw_in));
+        OTF_HIP(zero(o->dw_up, o->f, o->d, o->lddw_in));
+        OTF_HIP(zero(o->dw_down, o->d, o->f, o->lddw_down));
+        return OTF_OK;
+    }
+    if (!o->dy || !o->saved || !o->w_down || bad_ld(o->lddy, o->d) || bad_ld(o->ldw_down, o->f)) return OTF_EINVAL;
+    if (o->dx && (!o->w_gate || !o->w_up || bad_ld(o->ldw_in, o->d) || o->lddx < o->d)) return OTF_EINVAL;
+    if (o->dw_gate && (!o->x || bad_ld(o->ldx, o->d))) return OTF_EINVAL;
+    for (const void* p : {o->dy, o->x, o->w_gate, o->w_up, o->w_down, (const void*)o->dx})
+        if (misaligned(p, o->dtype)) return OTF_EINVAL;
+    if ((uintptr_t)o->saved % 16 || (uintptr_t)workspace % 16) return OTF_EINVAL;
+    size_t need = 0;
+    const int rs = backward_any(o, nullptr, &need, false, nullptr);
+    if (rs != OTF_OK) return rs;
+    if (need && (!workspace || workspace_bytes < need)) return OTF_EINVAL;
+    return backward_any(o, workspace, &need, true, s);
+}
+
+}  // extern "C"

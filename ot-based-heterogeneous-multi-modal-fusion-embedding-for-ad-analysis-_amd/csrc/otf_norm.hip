@@ -1,0 +1,766 @@
+// otf_norm.hip — dropout, layer norm and the residual sum with both, forward and backward.
+//
+// All of it is bound by HBM: each operand is read once and each result written once, rows
+// are held in registers between the statistics and the output, and the dropout mask is made
+// again from its counter instead of being stored (otf_rng.h).
+//
+//   dropout                y = [residual +] keep * x / (1 - p)
+//   layer norm             y = (x - mean) rstd w + b, statistics of a row in float32, the
+//                          variance from the centred values (a second pass over registers:
+//                          E[x^2] - mean^2 would cancel for rows with a large mean)
+//   its backward           c = dy w;  dx = rstd (c - mean(c) - xhat mean(c xhat));
+//                          dw = sum_rows dy xhat;  db = sum_rows dy
+//   residual norm          z = residual + dropout(x), y = LN(z), of z as it is stored, so
+//                          backward, which reads z, sees the same row; backward adds the
+//                          gradient that reaches z directly
+//
+// dw and db: every workgroup keeps float32 partials of its rows in registers and writes them
+// once; a second launch adds the partials in a fixed order (no atomics: the same bits every
+// call).
+#include "otf_rng.h"
+
+namespace otf {
+namespace {
+
+constexpr int kMaxHeldCols = 32768;   // 1024 threads x 4 chunks of 8
+
+struct NormArgs {
+    const void* x;       // forward: input; backward: the normalised input (x or z)
+    int64_t ldx;
+    const void* res;     // forward: residual; backward: dz (may be null)
+    int64_t ldr;
+    const void* dy;      // backward
+    int64_t lddy;
+    void* y;             // forward: y; backward: dx
+    int64_t ldy;
+    void* z;             // forward: z; backward: dresidual
+    int64_t ldz;
+    const void* w;
+    const void* b;
+    int wf32;            // weight and bias are float32 (else the input's type)
+    float* mean;
+    float* rstd;
+    float* partial;      // backward: [grid][2][cols]
+    void* dw;            // backward, one workgroup: written directly
+    void* db;
+    int64_t rows;
+    int cols;
+    float eps;
+    const int64_t* rng;
+    uint32_t threshold;
+    float scale;
+};
+
+__device__ __forceinline__ int chunk_valid(int cols, int col) { return cols - col < 8 ? cols - col : 8; }
+
+template <typename T>
+__device__ __forceinline__ void load_param8(const void* p, int wf32, int col, int valid, float (&v)[8]) {
+    if (wf32)
+        load8((const float*)p + col, valid, v);
+    else
+        load8((const T*)p + col, valid, v);
+}
+
+// Sum of NV values over the TPR threads of a row.  TPR = 64: one wave, no LDS.  Else one
+// barrier: `red` holds two generations of [wave][NV], and a wave can be at most one
+// reduction ahead of another.
+template <int TPR, int NV>
+__device__ __forceinline__ void row_sums(float (&s)[NV], float* red, int& gen) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) s[i] = wave_sum(s[i]);
+    if constexpr (TPR > 64) {
+        constexpr int NW = TPR / 64;
+        float* slot = red + gen * NW * NV;
+        const int wid = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) slot[wid * NV + i] = s[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) t += slot[w * NV + i];
+            s[i] = t;
+        }
+        gen ^= 1;
+    }
+}
+
+// ------------------------------------------------------------------------------- dropout
+// One thread a group of 8 columns.  FLAT: the tensor is one run of whole groups (no row
+// arithmetic).
+template <typename T, bool RES, bool FLAT>
+__global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, int64_t ldx,
+                                                      const T* __restrict__ res, int64_t ldr, T* __restrict__ y,
+                                                      int64_t ldy, uint64_t total, uint32_t groups, int cols,
+                                                      const int64_t* __restrict__ rng, uint32_t threshold,
+                                                      float scale) {
+    const uint64_t g = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (g >= total) return;
+    int64_t ox, orr, oy;
+    int valid = 8;
+    if constexpr (FLAT) {
+        ox = orr = oy = (int64_t)g * 8;
+    } else {
+        const uint64_t row = (total >> 32) ? g / groups : (uint64_t)((uint32_t)g / groups);
+        const int col = (int)(g - row * groups) * 8;
+        valid = chunk_valid(cols, col);
+        ox = (int64_t)row * ldx + col;
+        orr = (int64_t)row * ldr + col;
+        oy = (int64_t)row * ldy + col;
+    }
+    float v[8];
+    load8(x + ox, valid, v);
+    float r[8];
+    if constexpr (RES) load8(res + orr, valid, r);
+    drop8(v, g, drop_key(rng), threshold, scale);
+    if constexpr (RES)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+    store8(y + oy, valid, v);
+}
+
+// ---------------------------------------------------------------------------- layer norm
+// TPR threads a row, CH chunks of 8 columns a thread (chunk c of thread t: column
+// (c TPR + t) 8); a workgroup of max(TPR, 256) threads.
+template <typename T, typename TR, bool DROP, int TPR, int CH>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_forward_kernel(NormArgs a) {
+    constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
+    __shared__ float red[2 * (TPR / 64)];
+    int gen = 0;
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+    if (row >= a.rows) return;   // whole waves: RPB > 1 only where a wave is a row
+    const int cols = a.cols;
+    const T* x = (const T*)a.x + row * a.ldx;
+    float v[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + t) * 8;
+        load8(x + col, cols - col, v[c]);
+    }
+    if constexpr (DROP) {
+        const TR* res = (const TR*)a.res + row * a.ldr;
+        TR* z = (TR*)a.z + row * a.ldz;
+        const DropKey key = drop_key(a.rng);
+        const uint64_t first = (uint64_t)row * (uint32_t)((cols + 7) / 8);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + t) * 8;
+            if (col >= cols) continue;
+            float r[8];
+            load8(res + col, cols - col, r);
+            drop8(v[c], first + (uint32_t)(col / 8), key, a.threshold, a.scale);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[c][j] = col + j < cols ? (float)(TR)(v[c][j] + r[j]) : 0.0f;
+            store8(z + col, cols - col, v[c]);
+        }
+    }
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] += v[c][j];
+    row_sums<TPR, 1>(s, red, gen);
+    const float mean = s[0] / (float)cols;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = (c * TPR + t) * 8 + j < cols ? v[c][j] - mean : 0.0f;
+            s[0] += d * d;
+        }
+    row_sums<TPR, 1>(s, red, gen);
+    const float rstd = rsqrtf(s[0] / (float)cols + a.eps);
+    if (t == 0 && a.mean) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+    T* y = (T*)a.y + row * a.ldy;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + t) * 8;
+        if (col >= cols) continue;
+        float w[8], b[8];
+        if (a.w) load_param8<T>(a.w, a.wf32, col, cols - col, w);
+        if (a.b) load_param8<T>(a.b, a.wf32, col, cols - col, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float o = (v[c][j] - mean) * rstd;
+            if (a.w) o *= w[j];
+            if (a.b) o += b[j];
+            v[c][j] = o;
+        }
+        store8(y + col, cols - col, v[c]);
+    }
+}
+
+// Rows wider than kMaxHeldCols: one workgroup a row, the row read three times (its second
+// and third reading come from L2 / the memory-side cache).
+template <typename T, typename TR, bool DROP>
+__global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormArgs a) {
+    __shared__ float red[2 * 16];
+    int gen = 0;
+    const int64_t row = blockIdx.x;
+    const int cols = a.cols;
+    const T* x = (const T*)a.x + row * a.ldx;
+    TR* z = DROP ? (TR*)a.z + row * a.ldz : nullptr;
+    float s[1] = {0.0f};
+    for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
+        const int valid = (int)(cols - col < 8 ? cols - col : 8);
+        float v[8];
+        load8(x + col, valid, v);
+        if constexpr (DROP) {
+            float r[8];
+            load8((const TR*)a.res + row * a.ldr + col, valid, r);
+            drop8(v, (uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng), a.threshold,
+                  a.scale);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = j < valid ? (float)(TR)(v[j] + r[j]) : 0.0f;
+            store8(z + col, valid, v);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] += v[j];
+    }
+    row_sums<1024, 1>(s, red, gen);
+    const float mean = s[0] / (float)cols;
+    s[0] = 0.0f;
+    auto again = [&](int64_t col, int valid, float (&v)[8]) {   // this thread's own z, or x
+        if constexpr (DROP)
+            load8((const TR*)z + col, valid, v);
+        else
+            load8(x + col, valid, v);
+    };
+    for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
+        const int valid = (int)(cols - col < 8 ? cols - col : 8);
+        float v[8];
+        again(col, valid, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = j < valid ? v[j] - mean : 0.0f;
+            s[0] += d * d;
+        }
+    }
+    row_sums<1024, 1>(s, red, gen);
+    const float rstd = rsqrtf(s[0] / (float)cols + a.eps);
+    if (threadIdx.x == 0 && a.mean) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+    for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
+        const int valid = (int)(cols - col < 8 ? cols - col : 8);
+        float v[8], w[8], b[8];
+        again(col, valid, v);
+        if (a.w) load_param8<T>(a.w, a.wf32, (int)col, valid, w);
+        if (a.b) load_param8<T>(a.b, a.wf32, (int)col, valid, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float o = (v[j] - mean) * rstd;
+            if (a.w) o *= w[j];
+            if (a.b) o += b[j];
+            v[j] = o;
+        }
+        store8((T*)a.y + row * a.ldy + col, valid, v);
+    }
+}
+
+// One parameter gradient's partial sums, or (one workgroup) the gradient itself.
+template <typename T>
+__device__ __forceinline__ void store_param_grad(const NormArgs& a, int which, int col, const float (&s)[8]) {
+    const int valid = chunk_valid(a.cols, col);
+    if (gridDim.x == 1) {
+        void* out = which ? a.db : a.dw;
+        if (!out) return;
+        if (a.wf32)
+            store8((float*)out + col, valid, s);
+        else
+            store8((T*)out + col, valid, s);
+    } else {
+        store8(a.partial + ((int64_t)blockIdx.x * 2 + which) * a.cols + col, valid, s);
+    }
+}
+
+// Rows gridDim RPB apart.  WG: parameter gradients wanted.  TR: the type of z (= T without
+// the residual sum).
+template <typename T, typename TR, bool DROP, bool WG, int NT, int TPR, int CH>
+__global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
+    constexpr int RPB = NT / TPR;
+    __shared__ float red[TPR > 64 ? 4 * (TPR / 64) : 1];
+    __shared__ float comb[WG && RPB > 1 ? (RPB - 1) * 64 * 8 : 1];
+    int gen = 0;
+    const int t = threadIdx.x % TPR, part = threadIdx.x / TPR;
+    const int cols = a.cols;
+    float w[CH][8], gw[CH][8], gb[CH][8];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + t) * 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[c][j] = 1.0f, gw[c][j] = 0.0f, gb[c][j] = 0.0f;
+        if (a.w && col < cols) load_param8<T>(a.w, a.wf32, col, cols - col, w[c]);
+    }
+    const float inv = 1.0f / (float)cols;
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(a.rng);
+    for (int64_t row = (int64_t)blockIdx.x * RPB + part; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+        const TR* x = (const TR*)a.x + row * a.ldx;
+        const T* dy = (const T*)a.dy + row * a.lddy;
+        float v[CH][8], g[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + t) * 8;
+            load8(x + col, cols - col, v[c]);
+            load8(dy + col, cols - col, g[c]);
+        }
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + t) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float xh = col + j < cols ? (v[c][j] - mean) * rstd : 0.0f;
+                v[c][j] = xh;
+                if constexpr (WG) {
+                    gw[c][j] += g[c][j] * xh;
+                    gb[c][j] += g[c][j];
+                }
+                g[c][j] *= w[c][j];
+                s[0] += g[c][j];
+                s[1] += g[c][j] * xh;
+            }
+        }
+        row_sums<TPR, 2>(s, red, gen);
+        const float m1 = s[0] * inv, m2 = s[1] * inv;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int col = (c * TPR + t) * 8;
+            if (col >= cols) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[c][j] = rstd * (g[c][j] - m1 - v[c][j] * m2);
+            if constexpr (DROP) {
+                if (a.res) {
+                    float r[8];
+                    load8((const TR*)a.res + row * a.ldr + col, cols - col, r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[c][j] += r[j];
+                }
+                store8((TR*)a.z + row * a.ldz + col, cols - col, g[c]);
+                drop8(g[c], (uint64_t)row * (uint32_t)((cols + 7) / 8) + (uint32_t)(col / 8), key, a.threshold, a.scale);
+            }
+            store8((T*)a.y + row * a.ldy + col, cols - col, g[c]);
+        }
+    }
+    if constexpr (WG) {
+        if constexpr (RPB == 1) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int col = (c * TPR + t) * 8;
+                if (col >= cols) continue;
+                store_param_grad<T>(a, 0, col, gw[c]);
+                store_param_grad<T>(a, 1, col, gb[c]);
+            }
+        } else {   // the workgroup's waves joined through LDS, a chunk of one gradient at a time
+#pragma unroll
+            for (int i = 0; i < 2 * CH; ++i) {
+                float(&s)[8] = (i & 1) ? gb[i >> 1] : gw[i >> 1];
+                __syncthreads();
+                if (part > 0)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) comb[((part - 1) * 8 + j) * 64 + t] = s[j];
+                __syncthreads();
+                const int col = ((i >> 1) * TPR + t) * 8;
+                if (part == 0 && col < cols) {
+                    for (int p = 0; p < RPB - 1; ++p)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) s[j] += comb[(p * 8 + j) * 64 + t];
+                    store_param_grad<T>(a, i & 1, col, s);
+                }
+            }
+        }
+    }
+}
+
+// Rows wider than kMaxHeldCols: dx (and dresidual) by one workgroup a row.
+template <typename T, typename TR, bool DROP>
+__global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
+    __shared__ float red[2 * 16 * 2];
+    int gen = 0;
+    const int64_t row = blockIdx.x;
+    const int cols = a.cols;
+    const TR* x = (const TR*)a.x + row * a.ldx;
+    const T* dy = (const T*)a.dy + row * a.lddy;
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float m1 = 0.0f, m2 = 0.0f;
+    for (int pass = 0; pass < 2; ++pass) {
+        float s[2] = {0.0f, 0.0f};
+        for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
+            const int valid = (int)(cols - col < 8 ? cols - col : 8);
+            float v[8], g[8], w[8];
+            load8(x + col, valid, v);
+            load8(dy + col, valid, g);
+            if (a.w) load_param8<T>(a.w, a.wf32, (int)col, valid, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = j < valid ? (v[j] - mean) * rstd : 0.0f;
+                if (a.w) g[j] *= w[j];
+                s[0] += g[j];
+                s[1] += g[j] * v[j];
+            }
+            if (pass == 1) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = rstd * (g[j] - m1 - v[j] * m2);
+                if constexpr (DROP) {
+                    if (a.res) {
+                        float r[8];
+                        load8((const TR*)a.res + row * a.ldr + col, valid, r);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) g[j] += r[j];
+                    }
+                    store8((TR*)a.z + row * a.ldz + col, valid, g);
+                    drop8(g, (uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng),
+                          a.threshold, a.scale);
+                }
+                store8((T*)a.y + row * a.ldy + col, valid, g);
+            }
+        }
+        if (pass == 0) {
+            row_sums<1024, 2>(s, red, gen);
+            m1 = s[0] / (float)cols;
+            m2 = s[1] / (float)cols;
+        }
+    }
+}
+
+// Parameter gradients of rows wider than kMaxHeldCols: 64 chunks of 8 columns by 4 waves,
+// each wave every fourth row.
+template <typename T, typename TR>
+__global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
+    __shared__ float comb[3 * 64 * 16];
+    const int t = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = ((int64_t)blockIdx.x * 64 + t) * 8;
+    const int valid = col < a.cols ? (int)(a.cols - col < 8 ? a.cols - col : 8) : 0;
+    float s[2][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[0][j] = 0.0f, s[1][j] = 0.0f;
+    if (valid > 0)
+        for (int64_t row = part; row < a.rows; row += 4) {
+            const float mean = a.mean[row], rstd = a.rstd[row];
+            float v[8], g[8];
+            load8((const TR*)a.x + row * a.ldx + col, valid, v);
+            load8((const T*)a.dy + row * a.lddy + col, valid, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s[0][j] += g[j] * ((v[j] - mean) * rstd);
+                s[1][j] += g[j];
+            }
+        }
+    if (part > 0)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) comb[((part - 1) * 16 + i) * 64 + t] = s[i >> 3][i & 7];
+    __syncthreads();
+    if (part > 0 || valid <= 0) return;
+    for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i >> 3][i & 7] += comb[(p * 16 + i) * 64 + t];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        void* out = i ? a.db : a.dw;
+        if (!out) continue;
+        if (a.wf32)
+            store8((float*)out + col, valid, s[i]);
+        else
+            store8((T*)out + col, valid, s[i]);
+    }
+}
+
+// partial [groups][2][cols] -> dw (blockIdx.y = 0), db (1).  64 columns a workgroup, its 16
+// waves every 16th partial each, joined in wave order.
+template <typename TW>
+__global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restrict__ partial, int groups, int cols,
+                                                          TW* dw, TW* db) {
+    __shared__ float comb[16 * 64];
+    TW* out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const int t = threadIdx.x & 63, wid = threadIdx.x >> 6;
+    const int64_t col = (int64_t)blockIdx.x * 64 + t;
+    float s = 0.0f;
+    if (col < cols) {
+        const float* p = partial + (int64_t)blockIdx.y * cols + col;
+#pragma unroll 4
+        for (int g = wid; g < groups; g += 16) s += p[(int64_t)g * 2 * cols];
+    }
+    comb[wid * 64 + t] = s;
+    __syncthreads();
+    if (wid == 0 && col < cols) {
+#pragma unroll
+        for (int k = 1; k < 16; ++k) s += comb[k * 64 + t];
+        out[col] = (TW)s;
+    }
+}
+
+// ------------------------------------------------------------------------------ dispatch
+template <typename T, typename TR, bool DROP>
+hipError_t norm_forward(const NormArgs& a, hipStream_t s) {
+#define OTF_NF(TPR, CH) norm_forward_kernel<T, TR, DROP, TPR, CH><<<grid, TPR > 256 ? TPR : 256, 0, s>>>(a)
+    const int c = a.cols;
+    const bool wave = c <= 2048;
+    const unsigned grid = (unsigned)(wave ? (a.rows + 3) / 4 : a.rows);
+    if (c <= 512)
+        OTF_NF(64, 1);
+    else if (c <= 1024)
+        OTF_NF(64, 2);
+    else if (c <= 2048)
+        OTF_NF(64, 4);
+    else if (c <= 4096)
+        OTF_NF(256, 2);
+    else if (c <= 8192)
+        OTF_NF(256, 4);
+    else if (c <= 16384)
+        OTF_NF(1024, 2);
+    else if (c <= kMaxHeldCols)
+        OTF_NF(1024, 4);
+    else
+        norm_forward_long_kernel<T, TR, DROP><<<grid, 1024, 0, s>>>(a);
+#undef OTF_NF
+    return hipGetLastError();
+}
+
+// Workgroups of the backward pass, each of which leaves one partial of dw and db.
+int norm_backward_groups(int64_t rows, int64_t cols) {
+    if (cols > kMaxHeldCols) return 1;
+    const int64_t per = cols <= 2048 ? 4 : 1;
+    const int64_t want = (rows + per - 1) / per, most = cols <= 8192 ? 512 : 256;
+    return (int)(want < most ? want : most);
+}
+
+template <typename T, typename TR, bool DROP, bool WG>
+hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
+    const int c = a.cols;
+    if (c > kMaxHeldCols) {
+        norm_backward_long_kernel<T, TR, DROP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+        if (WG) norm_param_long_kernel<T, TR><<<(unsigned)((c - 1) / 512 + 1), 256, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    const int grid = norm_backward_groups(a.rows, c);
+#define OTF_NB(NT, TPR, CH) norm_backward_kernel<T, TR, DROP, WG, NT, TPR, CH><<<grid, NT, 0, s>>>(a)
+    if (c <= 512)
+        OTF_NB(256, 64, 1);
+    else if (c <= 1024)
+        OTF_NB(256, 64, 2);
+    else if (c <= 2048)
+        OTF_NB(256, 64, 4);
+    else if (c <= 4096)
+        OTF_NB(256, 256, 2);
+    else if (c <= 8192)
+        OTF_NB(256, 256, 4);
+    else if (c <= 16384)
+        OTF_NB(1024, 1024, 2);
+    else
+        OTF_NB(1024, 1024, 4);
+#undef OTF_NB
+    if (WG && grid > 1) {
+        const dim3 g((unsigned)((c + 63) / 64), 2);
+        if (a.wf32)
+            norm_param_kernel<float><<<g, 1024, 0, s>>>(a.partial, grid, c, (float*)a.dw, (float*)a.db);
+        else
+            norm_param_kernel<T><<<g, 1024, 0, s>>>(a.partial, grid, c, (T*)a.dw, (T*)a.db);
+    }
+    return hipGetLastError();
+}
+
+template <typename T, typename TR, bool DROP>
+hipError_t norm_backward(const NormArgs& a, hipStream_t s) {
+    return a.dw || a.db ? norm_backward_wg<T, TR, DROP, true>(a, s) : norm_backward_wg<T, TR, DROP, false>(a, s);
+}
+
+template <typename T>
+hipError_t dropout_launch(const void* x, int64_t ldx, const void* res, int64_t ldr, void* y, int64_t ldy,
+                          int64_t rows, int64_t cols, uint32_t threshold, float scale, const int64_t* rng,
+                          hipStream_t s) {
+    const uint32_t groups = (uint32_t)((cols + 7) / 8);
+    const uint64_t total = (uint64_t)rows * groups;
+    const bool flat = cols % 8 == 0 && ldx == cols && ldy == cols && (!res || ldr == cols);
+    const unsigned grid = (unsigned)((total + 255) / 256);
+#define OTF_DK(RES, FLAT)                                                                                     \
+    dropout_kernel<T, RES, FLAT><<<grid, 256, 0, s>>>((const T*)x, ldx, (const T*)res, ldr, (T*)y, ldy, total, \
+                                                      groups, (int)cols, rng, threshold, scale)
+    if (res) {
+        if (flat)
+            OTF_DK(true, true);
+        else
+            OTF_DK(true, false);
+    } else {
+        if (flat)
+            OTF_DK(false, true);
+        else
+            OTF_DK(false, false);
+    }
+#undef OTF_DK
+    return hipGetLastError();
+}
+
+bool type16_or_32(int32_t t) { return t == OTF_F32 || t == OTF_F16 || t == OTF_BF16; }
+size_t elem_size(int32_t t) { return t == OTF_F32 ? 4 : 2; }
+bool elem_aligned(const void* p, int32_t t) { return (uintptr_t)p % elem_size(t) == 0; }
+
+// what every call here checks: sizes within the kernels' index types, types, parameters
+int check_norm(int64_t rows, int64_t cols, int32_t dtype, int32_t rdtype, int32_t wdtype) {
+    if (rows < 0 || cols <= 0) return OTF_EINVAL;
+    if (!type16_or_32(dtype)) return OTF_EINVAL;
+    if (rdtype != dtype && rdtype != OTF_F32) return OTF_EINVAL;
+    if (wdtype != dtype && wdtype != OTF_F32) return OTF_EINVAL;
+    if (rows > INT32_MAX || cols > INT32_MAX - 8192) return OTF_EUNSUPPORTED;
+    return OTF_OK;
+}
+
+template <bool DROP, typename F> int by_type(int32_t dtype, int32_t rdtype, F f) {
+    hipError_t e;
+    if (dtype == OTF_F32)
+        e = f((float*)0, (float*)0);
+    else if (dtype == OTF_F16)
+        e = (DROP && rdtype == OTF_F32) ? f((_Float16*)0, (float*)0) : f((_Float16*)0, (_Float16*)0);
+    else
+        e = (DROP && rdtype == OTF_F32) ? f((__bf16*)0, (float*)0) : f((__bf16*)0, (__bf16*)0);
+    return check_hip(e);
+}
+
+}  // namespace
+}  // namespace otf
+
+using namespace otf;
+
+extern "C" {
+
+int otf_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* y, int64_t ldy, int64_t rows,
+                int64_t cols, int32_t dtype, double p, const int64_t* rng, otf_stream_t stream) {
+    uint32_t threshold;
+    float scale;
+    if (rows < 0 || cols < 0 || !type16_or_32(dtype) || !drop_params(p, threshold, scale)) return OTF_EINVAL;
+    if (rows == 0 || cols == 0) return OTF_OK;
+    if (!x || !y || !rng || ldx < cols || ldy < cols || (residual && ldr < cols)) return OTF_EINVAL;
+    if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || !elem_aligned(residual, dtype)) return OTF_EINVAL;
+    if ((uintptr_t)rng % 8) return OTF_EINVAL;
+    if (cols > INT32_MAX - 8 || rows > INT64_MAX / ((cols + 7) / 8)) return OTF_EUNSUPPORTED;
+    if (rows * ((cols + 7) / 8) > (int64_t)256 * INT32_MAX) return OTF_EUNSUPPORTED;
+    return by_type<false>(dtype, dtype, [&](auto* t, auto*) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return dropout_launch<T>(x, ldx, residual, ldr, y, ldy, rows, cols, threshold, scale, rng, (hipStream_t)stream);
+    });
+}
+
+int otf_layer_norm(const void* x, int64_t ldx, int32_t dtype, const void* weight, const void* bias, int32_t wdtype,
+                   double eps, int64_t rows, int64_t cols, void* y, int64_t ldy, float* mean, float* rstd,
+                   otf_stream_t stream) {
+    const int rc = check_norm(rows, cols, dtype, dtype, wdtype);
+    if (rc != OTF_OK) return rc;
+    if (!(eps >= 0.0) || (mean == nullptr) != (rstd == nullptr)) return OTF_EINVAL;
+    if (rows == 0) return OTF_OK;
+    if (!x || !y || ldx < cols || ldy < cols) return OTF_EINVAL;
+    if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || !elem_aligned(weight, wdtype) ||
+        !elem_aligned(bias, wdtype) || !elem_aligned(mean, OTF_F32) || !elem_aligned(rstd, OTF_F32))
+        return OTF_EINVAL;
+    NormArgs a{};
+    a.x = x, a.ldx = ldx, a.y = y, a.ldy = ldy, a.w = weight, a.b = bias, a.wf32 = wdtype == OTF_F32;
+    a.mean = mean, a.rstd = rstd, a.rows = rows, a.cols = (int)cols, a.eps = (float)eps;
+    return by_type<false>(dtype, dtype, [&](auto* t, auto*) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return norm_forward<T, T, false>(a, (hipStream_t)stream);
+    });
+}
+
+int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const void* residual, int64_t ldr,
+                               int32_t rdtype, const void* weight, const void* bias, int32_t wdtype, double eps,
+                               double p, const int64_t* rng, int64_t rows, int64_t cols, void* y, int64_t ldy,
+                               void* z, int64_t ldz, float* mean, float* rstd, otf_stream_t stream) {
+    const int rc = check_norm(rows, cols, dtype, rdtype, wdtype);
+    if (rc != OTF_OK) return rc;
+    NormArgs a{};
+    if (!(eps >= 0.0) || (mean == nullptr) != (rstd == nullptr) || !drop_params(p, a.threshold, a.scale))
+        return OTF_EINVAL;
+    if (rows == 0) return OTF_OK;
+    if (!x || !residual || !y || !z || !rng || ldx < cols || ldr < cols || ldy < cols || ldz < cols) return OTF_EINVAL;
+    if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || !elem_aligned(residual, rdtype) ||
+        !elem_aligned(z, rdtype) || !elem_aligned(weight, wdtype) || !elem_aligned(bias, wdtype) ||
+        !elem_aligned(mean, OTF_F32) || !elem_aligned(rstd, OTF_F32) || (uintptr_t)rng % 8)
+        return OTF_EINVAL;
+    a.x = x, a.ldx = ldx, a.res = residual, a.ldr = ldr, a.y = y, a.ldy = ldy, a.z = z, a.ldz = ldz;
+    a.w = weight, a.b = bias, a.wf32 = wdtype == OTF_F32, a.mean = mean, a.rstd = rstd, a.rng = rng;
+    a.rows = rows, a.cols = (int)cols, a.eps = (float)eps;
+    return by_type<true>(dtype, rdtype, [&](auto* t, auto* r) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        using TR = std::remove_pointer_t<decltype(r)>;
+        return norm_forward<T, TR, true>(a, (hipStream_t)stream);
+    });
+}
+
+size_t otf_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
+    if (rows <= 0 || cols <= 0 || cols > kMaxHeldCols) return 0;
+    const int g = norm_backward_groups(rows, cols);
+    return g > 1 ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;
+}
+
+// shared by the two backward entry points
+static int norm_backward_call(NormArgs& a, bool drop, int32_t dtype, int32_t rdtype, int32_t wdtype, int64_t rows,
+                              int64_t cols, void* workspace, size_t workspace_bytes, otf_stream_t stream) {
+    const int rc = check_norm(rows, cols, dtype, rdtype, wdtype);
+    if (rc != OTF_OK) return rc;
+    a.rows = rows, a.cols = (int)cols, a.wf32 = wdtype == OTF_F32, a.partial = (float*)workspace;
+    hipStream_t s = (hipStream_t)stream;
+    if (!elem_aligned(a.dw, wdtype) || !elem_aligned(a.db, wdtype) || !elem_aligned(a.w, wdtype)) return OTF_EINVAL;
+    if (rows == 0) {   // no row: the sums are zero
+        const int n = (int)cols;
+        const dim3 g((unsigned)((n + 63) / 64), 2);
+        if (!a.dw && !a.db) return OTF_OK;
+        if (a.wf32)
+            norm_param_kernel<float><<<g, 1024, 0, s>>>(nullptr, 0, n, (float*)a.dw, (float*)a.db);
+        else
+            norm_param_kernel<_Float16><<<g, 1024, 0, s>>>(nullptr, 0, n, (_Float16*)a.dw, (_Float16*)a.db);  // 0 is 0 in both 16-bit types
+        return check_hip(hipGetLastError());
+    }
+    if (!a.x || !a.dy || !a.y || !a.mean || !a.rstd || a.ldx < cols || a.lddy < cols || a.ldy < cols) return OTF_EINVAL;
+    if (!elem_aligned(a.x, rdtype) || !elem_aligned(a.dy, dtype) || !elem_aligned(a.y, dtype) ||
+        !elem_aligned(a.res, rdtype) || !elem_aligned(a.z, rdtype) || !elem_aligned(a.mean, OTF_F32) ||
+        !elem_aligned(a.rstd, OTF_F32))
+        return OTF_EINVAL;
+    const size_t need = (a.dw || a.db) ? otf_layer_norm_backward_workspace_size(rows, cols) : 0;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return OTF_EINVAL;
+    if (drop)
+        return by_type<true>(dtype, rdtype, [&](auto* t, auto* r) {
+            using T = std::remove_pointer_t<decltype(t)>;
+            using TR = std::remove_pointer_t<decltype(r)>;
+            return norm_backward<T, TR, true>(a, s);
+        });
+    return by_type<false>(dtype, dtype, [&](auto* t, auto*) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        return norm_backward<T, T, false>(a, s);
+    });
+}
+
+int otf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, int32_t dtype,
+                            const void* weight, int32_t wdtype, const float* mean, const float* rstd, int64_t rows,
+                            int64_t cols, void* dx, int64_t lddx, void* dweight, void* dbias, void* workspace,
+                            size_t workspace_bytes, otf_stream_t stream) {
+    NormArgs a{};
+    a.dy = dy, a.lddy = lddy, a.x = x, a.ldx = ldx, a.w = weight, a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd), a.y = dx, a.ldy = lddx, a.dw = dweight, a.db = dbias;
+    return norm_backward_call(a, false, dtype, dtype, wdtype, rows, cols, workspace, workspace_bytes, stream);
+}
+
+int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void* dz, int64_t lddz, const void* z,
+                                        int64_t ldz, int32_t dtype, int32_t rdtype, const void* weight,
+                                        int32_t wdtype, const float* mean, const float* rstd, double p,
+                                        const int64_t* rng, int64_t rows, int64_t cols, void* dx, int64_t lddx,
+                                        void* dresidual, int64_t lddr, void* dweight, void* dbias, void* workspace,
+                                        size_t workspace_bytes, otf_stream_t stream) {
+    NormArgs a{};
+    if (!drop_params(p, a.threshold, a.scale)) return OTF_EINVAL;
+    if (rows > 0 && (!rng || (uintptr_t)rng % 8 || !dresidual || lddr < cols || (dz && lddz < cols))) return OTF_EINVAL;
+    a.dy = dy, a.lddy = lddy, a.res = dz, a.ldr = lddz, a.x = z, a.ldx = ldz, a.w = weight;
+    a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.rng = rng;
+    a.y = dx, a.ldy = lddx, a.z = dresidual, a.ldz = lddr, a.dw = dweight, a.db = dbias;
+    return norm_backward_call(a, true, dtype, rdtype, wdtype, rows, cols, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -30,6 +30,7 @@ COMM_ID_BYTES = 128
 SK_RUNNING, SK_CONVERGED, SK_MAX_ITER, SK_NUMERICAL_BREAK, SK_TIMEOUT = 0, 1, 2, 3, 4
 STATUS_NAMES = {0: "running", 1: "converged", 2: "max_iter", 3: "numerical_break",
                 4: "timeout"}
+ACTIVATIONS = {"silu": 0, "gelu": 1}
 ENGINE_AUTO, ENGINE_STREAM, ENGINE_RESIDENT, ENGINE_TILED, ENGINE_SWEEP, ENGINE_GATHER, ENGINE_MESH = (
     0, 1, 2, 3, 4, 5, 6)
 ENGINES = {"auto": ENGINE_AUTO, "stream": ENGINE_STREAM, "resident": ENGINE_RESIDENT,
@@ -72,6 +73,19 @@ class EmdProblem(ctypes.Structure):
                 ("n", ctypes.c_int32), ("m", ctypes.c_int32)]
 
 
+class FfnArgs(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("d", ctypes.c_int64), ("f", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64),
+                ("w_gate", ctypes.c_void_p), ("w_up", ctypes.c_void_p), ("ldw_in", ctypes.c_int64),
+                ("w_down", ctypes.c_void_p), ("ldw_down", ctypes.c_int64),
+                ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("saved", ctypes.c_void_p),
+                ("dy", ctypes.c_void_p), ("lddy", ctypes.c_int64),
+                ("dx", ctypes.c_void_p), ("lddx", ctypes.c_int64),
+                ("dw_gate", ctypes.c_void_p), ("dw_up", ctypes.c_void_p), ("lddw_in", ctypes.c_int64),
+                ("dw_down", ctypes.c_void_p), ("lddw_down", ctypes.c_int64)]
+
+
 EMD_STATUS = {0: "optimal", 1: "max_iter", 2: "infeasible", 3: "unbounded"}
 
 INFO_FIELDS = ("stop", "last_good", "niter", "status", "n_err", "break_iter", "engine", "stalled",
@@ -81,6 +95,7 @@ INFO_INT32S = len(INFO_FIELDS)  # otf_sinkhorn_info is 9 x int32
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
+_dbl = ctypes.c_double
 _SIGS = {
     "otf_version": (ctypes.c_char_p, []),
     "otf_cost_pairwise": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp,
@@ -162,6 +177,21 @@ _SIGS = {
     "otf_emd_max_nodes": (ctypes.c_int, []),
     "otf_emd_lds_nodes": (ctypes.c_int, []),
     "otf_emd_solve": (ctypes.c_int, [_i32, ctypes.POINTER(EmdProblem), _i64, _vp, _vp]),
+    "otf_dropout": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i32, _dbl, _vp, _vp]),
+    "otf_layer_norm": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _i32, _dbl, _i64, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "otf_layer_norm_backward_workspace_size": (ctypes.c_size_t, [_i64, _i64]),
+    "otf_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i64, _i64, _vp,
+                                               _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "otf_dropout_add_layer_norm": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _dbl, _dbl, _vp,
+                                                  _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    "otf_dropout_add_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _i32,
+                                                           _vp, _vp, _dbl, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                                           _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "otf_gated_ffn_saved_size": (ctypes.c_size_t, [_i64, _i64, _i32]),
+    "otf_gated_ffn_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
+    "otf_gated_ffn": (ctypes.c_int, [ctypes.POINTER(FfnArgs), _vp, ctypes.c_size_t, _vp]),
+    "otf_gated_ffn_backward_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(FfnArgs)]),
+    "otf_gated_ffn_backward": (ctypes.c_int, [ctypes.POINTER(FfnArgs), _vp, ctypes.c_size_t, _vp]),
     "otf_gw_workspace_size": (ctypes.c_size_t, [ctypes.c_int32, ctypes.POINTER(GwProblem)]),
     "otf_gw_solve": (ctypes.c_int, [ctypes.c_int32, ctypes.POINTER(GwProblem),
                                     ctypes.POINTER(GwOpts), ctypes.c_void_p, ctypes.c_void_p,

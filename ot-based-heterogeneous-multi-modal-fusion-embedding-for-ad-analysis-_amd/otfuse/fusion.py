@@ -13,6 +13,10 @@ torch.  Here the whole block stays on the device and in HIP kernels:
     stalled device barrier (decided on the device: no host sync).
 
 ``group_features_by_label`` mirrors MRI_PET_OT_nojax.py:884-903 for the per-epoch path.
+
+``FeedForwardBlock`` is the part of SelfAttentionBlock after its attention
+(MRI_PET_OT_nojax.py:523-549) on the kernels of ``layers``: residual sums with dropout and
+layer norm, and a gated feed-forward part between them.
 """
 from __future__ import annotations
 
@@ -20,7 +24,7 @@ import numpy as np
 import torch
 import torch.nn.functional as F
 
-from . import ops
+from . import layers, ops
 from .pot import feature_coupling_pot_device
 
 
@@ -100,6 +104,39 @@ def ot_alignment_loss(mri_fused: torch.Tensor, pet_fused: torch.Tensor,
         ot_loss, ot_mri_from_pet, T = _OTAlignLoss.apply(mri_fused, pet_fused, T_feature_pet2mri,
                                                          None, False)
     return ot_loss, ot_mri_from_pet, T
+
+
+class FeedForwardBlock(torch.nn.Module):
+    """What follows the attention in the fusion block (MRI_PET_OT_nojax.py:523-549): residual sum,
+    dropout and norm, then the feed-forward part with its own.
+
+        h = LN1(residual + dropout(attended))
+        out = LN2(h + dropout(gated_feed_forward(h)))
+
+    Its output feeds the classifier and ``ot_alignment_loss``.  ``rng`` (layers.rng_state) is
+    this step's state: the block's two dropouts take its offset and the next one; it is not
+    read in eval mode."""
+
+    def __init__(self, d: int, f: int, p: float = 0.1, activation: str = "silu", eps: float = 1e-5,
+                 device=None, dtype=None):
+        super().__init__()
+        kw = dict(device=device, dtype=dtype)
+        self.p, self.activation, self.eps = p, activation, eps
+        self.norm1 = torch.nn.LayerNorm(d, eps, **kw)
+        self.norm2 = torch.nn.LayerNorm(d, eps, **kw)
+        self.gate = torch.nn.Linear(d, f, bias=False, **kw)
+        self.up = torch.nn.Linear(d, f, bias=False, **kw)
+        self.down = torch.nn.Linear(f, d, bias=False, **kw)
+        self.register_buffer("next_offset", torch.tensor([0, 1], device=device), persistent=False)
+
+    def forward(self, attended: torch.Tensor, residual: torch.Tensor, rng: torch.Tensor | None = None) -> torch.Tensor:
+        p = self.p if self.training else 0.0
+        h, _ = layers.dropout_add_layer_norm(attended, residual, self.norm1.weight, self.norm1.bias, p,
+                                             rng if p else None, self.eps)
+        ffn = layers.gated_feed_forward(h, self.gate.weight, self.up.weight, self.down.weight, self.activation)
+        out, _ = layers.dropout_add_layer_norm(ffn, h, self.norm2.weight, self.norm2.bias, p,
+                                               rng + self.next_offset if p else None, self.eps)
+        return out
 
 
 def group_features_by_label(y, p, max_samples_per_label=None):
