@@ -357,6 +357,199 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
         }
 }
 
+// ---- the tiled product, 256 x 256 -----------------------------------------------------------
+// 16-bit operands, eight waves in 2 (m) x 4 (n), each 2 x 64 rows by 2 x 32 columns: 128
+// accumulator registers a lane.  Each operand's tile is two half-tiles of 16 KB; two K-tiles of
+// four half-tiles fill 128 KB of LDS.  A K-tile runs as four phases, one quadrant of the result
+// each (A0 B0, A0 B1, A1 B1, A1 B0), so a phase reads only the fragments that the registers do not
+// hold; each phase puts one half-tile of the next K-tile in flight, in the order of first use
+// (A0, B0, B1, A1), and waits for all but the two latest: what the next phase reads has landed
+// and two half-tiles stay in flight across every barrier.  The two wave groups (m) run one
+// barrier apart, so on every SIMD one wave's MFMAs cover the other's LDS reads and loads.
+template <int OFF> __device__ __forceinline__ void read_tr4(const uint32_t (&p)[4], s16x4 (&f)[4][2][2]) {
+    // the wait is part of the block: nothing after it can use a register whose read is under way
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %16 offset:%20\n\tds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %2, %16 offset:%22\n\tds_read_b64_tr_b16 %3, %16 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %4, %17 offset:%20\n\tds_read_b64_tr_b16 %5, %17 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %6, %17 offset:%22\n\tds_read_b64_tr_b16 %7, %17 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %8, %18 offset:%20\n\tds_read_b64_tr_b16 %9, %18 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %10, %18 offset:%22\n\tds_read_b64_tr_b16 %11, %18 offset:%23\n\t"
+        "ds_read_b64_tr_b16 %12, %19 offset:%20\n\tds_read_b64_tr_b16 %13, %19 offset:%21\n\t"
+        "ds_read_b64_tr_b16 %14, %19 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]),
+          "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1]), "=&v"(f[2][0][0]), "=&v"(f[2][0][1]),
+          "=&v"(f[2][1][0]), "=&v"(f[2][1][1]), "=&v"(f[3][0][0]), "=&v"(f[3][0][1]), "=&v"(f[3][1][0]),
+          "=&v"(f[3][1][1])
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF), "n"(OFF + 1024), "n"(OFF + 8192), "n"(OFF + 9216)
+        : "memory");
+}
+template <int OFF> __device__ __forceinline__ void read_tr2(const uint32_t (&p)[2], s16x4 (&f)[2][2][2]) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %4, %9 offset:%10\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+        "ds_read_b64_tr_b16 %6, %9 offset:%12\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]),
+          "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1])
+        : "v"(p[0]), "v"(p[1]), "n"(OFF), "n"(OFF + 1024), "n"(OFF + 8192), "n"(OFF + 9216)
+        : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <typename T, bool TRA, bool TRB, int EPI>
+__global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
+    static_assert(sizeof(T) == 2, "16-bit operands");
+    constexpr int HT = 128 * kTileBytes, BUF = 4 * HT;   // half-tiles A0, A1, B0, B1
+    using TA = Tile<T, TRA, 128, 512>;
+    using TB = Tile<T, TRB, 128, 512>;
+    using F = typename Frag<T>::type;
+    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid >> 2, wn = wid & 3;
+
+    const int tiles = a.tiles_m * a.tiles_n, z = blockIdx.y % a.batch, split = blockIdx.y / a.batch;
+    int tm, tn;
+    tile_of(blockIdx.x, tiles, a.tiles_m, a.tiles_n, tm, tn);
+    const int m0 = tm * 256, n0 = EPI == kGatedForward ? tn * 128 : tn * 256;
+
+    TA ta;
+    TB tb;
+    ta.init(a.a.ld);
+    tb.init(a.b.ld);
+    const int64_t am = TRA ? (int64_t)m0 * 2 : (int64_t)m0 * a.a.ld, ah = TRA ? 256 : 128 * a.a.ld;
+    const int64_t bn = TRB ? (int64_t)n0 * 2 : (int64_t)n0 * a.b.ld, bh = TRB ? 256 : 128 * a.b.ld;
+    const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
+    const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
+    auto stage_a = [&](int h, int kt, int buf) {
+        const int seg = kt >= nk ? 1 : 0;
+        ta.stage(a.a.p[a.batch > 1 ? z : seg] + am + h * ah, a.a.ld, a.a.mn - m0 - h * 128, a.a.k, kt - seg * nk,
+                 smem + buf * BUF + h * HT);
+    };
+    auto stage_b = [&](int h, int kt, int buf) {
+        const int seg = kt >= nk ? 1 : 0;
+        if constexpr (EPI == kGatedForward)
+            tb.stage(a.b.p[h] + bn, a.b.ld, a.b.mn - n0, a.b.k, kt, smem + buf * BUF + (2 + h) * HT);
+        else
+            tb.stage(a.b.p[seg] + bn + h * bh, a.b.ld, a.b.mn - n0 - h * 128, a.b.k, kt - seg * nk,
+                     smem + buf * BUF + (2 + h) * HT);
+    };
+
+    // layout T: this lane's LDS address of each 16-column block (first k, first half of a K-tile)
+    uint32_t pa[4], pb[2];
+    {
+        const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
+        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+        auto at = [&](int r0) {
+            return base + k * 256 + (((r0 / 8 + ((i & 3) >> 1)) ^ swz_t<T, 128>(k)) << 4) + (i & 1) * 8;
+        };
+#pragma unroll
+        for (int t = 0; t < 4; ++t) pa[t] = at(wm * 64 + t * 16);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) pb[u] = at(wn * 32 + u * 16);
+    }
+    union FA {
+        s16x4 h[4][2][2];
+        F f[4][2];
+    } fa;
+    union FB {
+        s16x4 h[2][2][2];
+        F f[2][2];
+    } fb[2];
+    auto read_a = [&](int buf, auto half) {
+        constexpr int H = decltype(half)::value;
+        if constexpr (TRA) {
+            const uint32_t p[4] = {pa[0] + buf * BUF, pa[1] + buf * BUF, pa[2] + buf * BUF, pa[3] + buf * BUF};
+            read_tr4<H * HT>(p, fa.h);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) fa.f[t][s] = TA::frag(smem + buf * BUF + H * HT, wm * 64 + t * 16, s, lane);
+        }
+    };
+    auto read_b = [&](int buf, auto half) {
+        constexpr int H = decltype(half)::value;
+        if constexpr (TRB) {
+            const uint32_t p[2] = {pb[0] + buf * BUF, pb[1] + buf * BUF};
+            read_tr2<(2 + H) * HT>(p, fb[H].h);
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) fb[H].f[u][s] = TB::frag(smem + buf * BUF + (2 + H) * HT, wn * 32 + u * 16, s, lane);
+        }
+    };
+    f32x4 acc[2][2][4][2];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i >> 4][(i >> 3) & 1][(i >> 1) & 3][i & 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto quadrant = [&](auto ha, auto hb) {
+        constexpr int A = decltype(ha)::value, B = decltype(hb)::value;
+        __builtin_amdgcn_s_barrier();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) acc[A][B][t][u] = Frag<T>::mma(fb[B].f[u][s], fa.f[t][s], acc[A][B][t][u]);
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+
+    stage_a(0, k0, 0);
+    stage_b(0, k0, 0);
+    stage_b(1, k0, 0);
+    stage_a(1, k0, 0);
+    wait_loads<4>();
+    __builtin_amdgcn_s_barrier();
+    const int group = __builtin_amdgcn_readfirstlane(wm);
+    if (group == 1) __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    for (int kt = k0; kt < k1; ++kt) {
+        const int buf = (kt - k0) & 1;
+        const bool more = kt + 1 < k1;
+        if (more) stage_a(0, kt + 1, buf ^ 1);
+        read_b(buf, I0{});
+        read_a(buf, I0{});
+        if (more)
+            wait_loads<4>();   // B1 of this K-tile
+        else
+            wait_loads<2>();
+        quadrant(I0{}, I0{});
+        if (more) stage_b(0, kt + 1, buf ^ 1);
+        read_b(buf, I1{});
+        if (more)
+            wait_loads<4>();   // A1
+        else
+            wait_loads<0>();
+        quadrant(I0{}, I1{});
+        if (more) stage_b(1, kt + 1, buf ^ 1);
+        read_a(buf, I1{});
+        quadrant(I1{}, I1{});
+        if (more) {
+            stage_a(1, kt + 1, buf ^ 1);
+            wait_loads<4>();   // A0 and B0 of the next
+        }
+        quadrant(I1{}, I0{});
+    }
+    if (group == 0) __builtin_amdgcn_s_barrier();   // both groups pass the same number of barriers
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int m = m0 + h * 128 + wm * 64 + t * 16 + (lane & 15), n = n0 + wn * 32 + u * 16 + (lane >> 4) * 4;
+                finish4<T, EPI>(a, z, split, m, n, n + 128, acc[h][0][t][u], acc[h][1][t][u]);
+            }
+}
+
 // slabs [splits][batch][M][ldp] added in order and rounded once
 template <typename T>
 __global__ __launch_bounds__(256) void ffn_join_kernel(const float* __restrict__ slab, int splits, int batch, int64_t M,
@@ -512,8 +705,8 @@ struct Product {
 
 constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 
-// Tile 128 x 128 where that fills the chip, else 64 x 64; K split into slabs where even the
-// small tiles leave most of it idle.
+// Tile 256 x 256 (16-bit operands) where that fills the chip, else 128 x 128, else 64 x 64; K
+// split into slabs where even the small tiles leave most of it idle.
 struct Plan {
     int tm, tn, splits;
 };
@@ -523,7 +716,7 @@ Plan plan_product(const Product& p, int elem) {
         const int64_t m = (a.M + t - 1) / t, n = p.epi == kGatedForward ? (2 * (int64_t)a.N + t - 1) / t : (a.N + t - 1) / t;
         return m * n * a.batch;
     };
-    const int side = tiles(128) >= kCus ? 128 : 64;
+    const int side = elem == 2 && tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
     int splits = 1;
     if (p.epi == kStore) {
         const int64_t ktiles = (int64_t)(a.a.k + kTileBytes / elem - 1) / (kTileBytes / elem) * a.segments, t = tiles(side);
@@ -542,7 +735,9 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     const int cols = EPI == kGatedForward ? q.tn / 2 : q.tn;
     a.tiles_n = (a.N + cols - 1) / cols;
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
-    if (q.tm == 128)
+    if (q.tm == 256) {
+        if constexpr (sizeof(T) == 2) ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
+    } else if (q.tm == 128)
         ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
     else
         ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, EPI><<<grid, 256, 0, s>>>(a);

@@ -315,6 +315,26 @@ def test_gated_feed_forward(dev, dt, act, rows, d, f):
     assert all(torch.equal(p, q) for p, q in zip(grads, again))
 
 
+@pytest.mark.parametrize("dt,act,rows,d,f", [("bf16", "gelu", 4200, 4100, 4110), ("f16", "silu", 4097, 4104, 4352)])
+def test_gated_feed_forward_large_tiles(dev, dt, act, rows, d, f):
+    """Every product in whole and ragged tiles of the largest size, odd widths among them."""
+    t = T[dt]
+    from otfuse import layers
+    g = torch.Generator(device=dev).manual_seed(1)
+    r = lambda k, *s: (torch.randn(*s, device=dev, generator=g) * k).to(t).requires_grad_(True)
+    args = [r(1.0, rows, d), r(d ** -0.5, f, d), r(d ** -0.5, f, d), r(f ** -0.5, d, f)]
+    dy = r(1.0, rows, d).detach()
+    y = layers.gated_feed_forward(*args, activation=act)
+    grads = torch.autograd.grad(y, args, dy)
+    ref = plain.gated_feed_forward(*(v.detach().double() for v in args), act, dy.double())
+    depth = 2 * (d + f) + rows + 16
+    _close(y, ref[0], 3, t, depth)
+    for got, want, n in zip(grads, ref[1:], (7, 7, 7, 3)):
+        _close(got, want, n, t, depth)
+    again = torch.autograd.grad(layers.gated_feed_forward(*args, activation=act), args, dy)
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("rows", [4, 60])
 def test_gated_feed_forward_views(dev, dt, rows):
