@@ -361,10 +361,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 // 16-bit operands, eight waves in 2 (m) x 4 (n), each 2 x 64 rows by 2 x 32 columns: 128
 // accumulator registers a lane.  Each operand's tile is two half-tiles of 16 KB; two K-tiles of
 // four half-tiles fill 128 KB of LDS.  A K-tile runs as four phases, one quadrant of the result
-// each (A0 B0, A0 B1, A1 B1, A1 B0), so a phase reads only the fragments that the registers do not
-// hold; each phase puts one half-tile of the next K-tile in flight, in the order of first use
-// (A0, B0, B1, A1), and waits for all but the two latest: what the next phase reads has landed
-// and two half-tiles stay in flight across every barrier.  The two wave groups (m) run one
+// each (A0 B0, A0 B1, A1 B1, A1 B0; B's halves the other way round in every second K-tile), so a
+// phase reads only the fragments that the registers do not hold, 8, 4, 8 and 4 of them.  Each
+// phase puts one half-tile in flight, up to two K-tiles ahead.  The two wave groups (m) run one
 // barrier apart, so on every SIMD one wave's MFMAs cover the other's LDS reads and loads.
 template <int OFF> __device__ __forceinline__ void read_tr4(const uint32_t (&p)[4], s16x4 (&f)[4][2][2]) {
     // the wait is part of the block: nothing after it can use a register whose read is under way
@@ -502,43 +501,50 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
 
-    stage_a(0, k0, 0);
+    // K-tile kt of parity P takes B's half P first.  A half-tile is restaged, for the K-tile after
+    // the next, two phases after its last read: the other group's reads of the phase before may
+    // still be under way.  Every phase issues one half-tile and lets five stay in flight.  Past
+    // the end of K the loads bring zeros that nothing reads, so the counts hold to the last phase.
+    auto k_tile = [&](int kt, auto parity) {
+        constexpr int P = decltype(parity)::value;
+        using First = std::integral_constant<int, P>;
+        using Second = std::integral_constant<int, 1 - P>;
+        stage_a(1, kt + 1, 1 - P);
+        read_a(P, I0{});
+        wait_loads<10>();
+        quadrant(I0{}, First{});
+        stage_b(P, kt + 2, P);
+        read_b(P, Second{});
+        wait_loads<10>();
+        quadrant(I0{}, Second{});
+        stage_a(0, kt + 2, P);
+        read_a(P, I1{});
+        wait_loads<10>();
+        quadrant(I1{}, Second{});
+        stage_b(1 - P, kt + 2, P);
+        read_b(1 - P, Second{});   // the next K-tile's first half, into the registers this one is done with
+        wait_loads<10>();
+        quadrant(I1{}, First{});
+    };
     stage_b(0, k0, 0);
+    stage_a(0, k0, 0);
     stage_b(1, k0, 0);
     stage_a(1, k0, 0);
-    wait_loads<4>();
+    stage_b(1, k0 + 1, 1);
+    stage_a(0, k0 + 1, 1);
+    stage_b(0, k0 + 1, 1);
+    wait_loads<10>();   // B0 and A0
     __builtin_amdgcn_s_barrier();
     const int group = __builtin_amdgcn_readfirstlane(wm);
     if (group == 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    for (int kt = k0; kt < k1; ++kt) {
-        const int buf = (kt - k0) & 1;
-        const bool more = kt + 1 < k1;
-        if (more) stage_a(0, kt + 1, buf ^ 1);
-        read_b(buf, I0{});
-        read_a(buf, I0{});
-        if (more)
-            wait_loads<4>();   // B1 of this K-tile
-        else
-            wait_loads<2>();
-        quadrant(I0{}, I0{});
-        if (more) stage_b(0, kt + 1, buf ^ 1);
-        read_b(buf, I1{});
-        if (more)
-            wait_loads<4>();   // A1
-        else
-            wait_loads<0>();
-        quadrant(I0{}, I1{});
-        if (more) stage_b(1, kt + 1, buf ^ 1);
-        read_a(buf, I1{});
-        quadrant(I1{}, I1{});
-        if (more) {
-            stage_a(1, kt + 1, buf ^ 1);
-            wait_loads<4>();   // A0 and B0 of the next
-        }
-        quadrant(I1{}, I0{});
+    read_b(0, I0{});
+    for (int kt = k0; kt < k1; kt += 2) {
+        k_tile(kt, I0{});
+        if (kt + 1 < k1) k_tile(kt + 1, I1{});
     }
     if (group == 0) __builtin_amdgcn_s_barrier();   // both groups pass the same number of barriers
+    wait_loads<0>();
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
