@@ -56,13 +56,17 @@ template <> struct Frag<float> {
 
 // ---- activations ------------------------------------------------------------------------
 enum { kSilu = 0, kGelu = 1 };
+// one exponential and one reciprocal instruction, each within an ulp or two of float32
+__device__ __forceinline__ float sigmoid(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
+}
 __device__ __forceinline__ float act_value(int act, float g) {
-    if (act == kSilu) return g / (1.0f + expf(-g));
+    if (act == kSilu) return g * sigmoid(g);
     return 0.5f * g * erfcf(-0.70710678118654752f * g);
 }
 __device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
     if (act == kSilu) {
-        const float s = 1.0f / (1.0f + expf(-g));
+        const float s = sigmoid(g);
         a = g * s;
         da = s * (1.0f + g * (1.0f - s));
     } else {
@@ -271,6 +275,15 @@ __device__ __forceinline__ void tile_of(int id, int count, int tiles_m, int tile
     tn = in / rows;
 }
 
+// A kernel argument that a loop selects by a run-time index: in registers, so that the loop does
+// not load it again
+__device__ __forceinline__ const char* held(const char* p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("" : "+s"(p));
+#endif
+    return p;
+}
+
 // ---- the tiled product -----------------------------------------------------------------
 // TM x TN tile (B in two halves of TN / 2), WGM x WGN waves; K-tiles double-buffered: the
 // next one is on its way while this one's MFMAs run, one barrier a K-tile.
@@ -298,12 +311,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 
     const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
     const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
+    const char *pa0 = held(a.a.p[a.batch > 1 ? z : 0] + am), *pa1 = held(a.a.p[1] + am);   // a batch has one segment
+    const char *pb0 = held(a.b.p[0] + bn), *pb1 = held(a.b.p[1] + bn);
     auto stage = [&](int kt, int buf) {
         const int seg = kt >= nk ? 1 : 0, k = kt - seg * nk;
         char* dst = smem + buf * BUF;
-        ta.stage(a.a.p[a.batch > 1 ? z : seg] + am, a.a.ld, a.a.mn - m0, a.a.k, k, dst);
-        const char* b0 = a.b.p[EPI == kGatedForward ? 0 : seg] + bn;
-        const char* b1 = EPI == kGatedForward ? a.b.p[1] + bn : b0 + bh;
+        ta.stage(seg ? pa1 : pa0, a.a.ld, a.a.mn - m0, a.a.k, k, dst);
+        const char* b0 = EPI != kGatedForward && seg ? pb1 : pb0;
+        const char* b1 = EPI == kGatedForward ? pb1 : b0 + bh;
         tb.stage(b0, a.b.ld, a.b.mn - n0, a.b.k, k, dst + TA::BYTES);
         tb.stage(b1, a.b.ld, EPI == kGatedForward ? a.b.mn - n0 : a.b.mn - n0 - TH, a.b.k, k, dst + TA::BYTES + TB::BYTES);
     };
@@ -421,18 +436,20 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     const int64_t bn = TRB ? (int64_t)n0 * 2 : (int64_t)n0 * a.b.ld, bh = TRB ? 256 : 128 * a.b.ld;
     const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
     const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
+    const char *pa0 = held(a.a.p[a.batch > 1 ? z : 0] + am), *pa1 = held(a.a.p[1] + am);   // a batch has one segment
+    const char *pb0 = held(a.b.p[0] + bn), *pb1 = held(a.b.p[1] + bn);
     auto stage_a = [&](int h, int kt, int buf) {
-        const int seg = kt >= nk ? 1 : 0;
-        ta.stage(a.a.p[a.batch > 1 ? z : seg] + am + h * ah, a.a.ld, a.a.mn - m0 - h * 128, a.a.k, kt - seg * nk,
-                 smem + buf * BUF + h * HT);
+        const bool seg = kt >= nk && a.segments > 1;
+        ta.stage((seg ? pa1 : pa0) + h * ah, a.a.ld, a.a.mn - m0 - h * 128, a.a.k, seg ? kt - nk : kt, smem + buf * BUF + h * HT);
     };
     auto stage_b = [&](int h, int kt, int buf) {
-        const int seg = kt >= nk ? 1 : 0;
-        if constexpr (EPI == kGatedForward)
-            tb.stage(a.b.p[h] + bn, a.b.ld, a.b.mn - n0, a.b.k, kt, smem + buf * BUF + (2 + h) * HT);
-        else
-            tb.stage(a.b.p[seg] + bn + h * bh, a.b.ld, a.b.mn - n0 - h * 128, a.b.k, kt - seg * nk,
-                     smem + buf * BUF + (2 + h) * HT);
+        char* dst = smem + buf * BUF + (2 + h) * HT;
+        if constexpr (EPI == kGatedForward) {
+            tb.stage(h ? pb1 : pb0, a.b.ld, a.b.mn - n0, a.b.k, kt, dst);
+        } else {
+            const bool seg = kt >= nk && a.segments > 1;
+            tb.stage((seg ? pb1 : pb0) + h * bh, a.b.ld, a.b.mn - n0 - h * 128, a.b.k, seg ? kt - nk : kt, dst);
+        }
     };
 
     // layout T: this lane's LDS address of each 16-column block (first k, first half of a K-tile)
@@ -509,20 +526,24 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
         constexpr int P = decltype(parity)::value;
         using First = std::integral_constant<int, P>;
         using Second = std::integral_constant<int, 1 - P>;
-        stage_a(1, kt + 1, 1 - P);
+        if constexpr (TRA) stage_a(1, kt + 1, 1 - P);
         read_a(P, I0{});
+        if constexpr (!TRA) stage_a(1, kt + 1, 1 - P);
         wait_loads<10>();
         quadrant(I0{}, First{});
-        stage_b(P, kt + 2, P);
+        if constexpr (TRB) stage_b(P, kt + 2, P);
         read_b(P, Second{});
+        if constexpr (!TRB) stage_b(P, kt + 2, P);
         wait_loads<10>();
         quadrant(I0{}, Second{});
-        stage_a(0, kt + 2, P);
+        if constexpr (TRA) stage_a(0, kt + 2, P);
         read_a(P, I1{});
+        if constexpr (!TRA) stage_a(0, kt + 2, P);
         wait_loads<10>();
         quadrant(I1{}, Second{});
-        stage_b(1 - P, kt + 2, P);
-        read_b(1 - P, Second{});   // the next K-tile's first half, into the registers this one is done with
+        if constexpr (TRB) stage_b(1 - P, kt + 2, P);
+        read_b(1 - P, Second{});
+        if constexpr (!TRB) stage_b(1 - P, kt + 2, P);
         wait_loads<10>();
         quadrant(I1{}, First{});
     };
