@@ -12,8 +12,10 @@
 // as zero from the buffer descriptor's range check, so ragged edges cost no branch.  Layout T
 // is transposed on the way from LDS to registers (ds_read_b64_tr_b16).
 //
-// All sums are float32 in the accumulators.  h, and g and u for the backward pass, are kept in
-// the operands' type: one rounding each, which the products that read them need anyway.
+// All sums are float32 in the accumulators.  h, dg and du are rounded to the operands' type, which
+// the products that read them need; g and u are kept in float32 for the backward pass, where their
+// rounding would meet dg's and du's own (gradients of 16-bit operands then err by 1.4 times their
+// final rounding instead of 1.8; at 8192 x 4096 x 11264 the wider buffers cost 2 % of a step).
 #include "otf_rng.h"
 
 namespace otf {
@@ -152,6 +154,18 @@ template <typename T, bool TR, int R, int NT> struct Tile {
         }
 #endif
     }
+    // the same with the range worked out by the caller: `bytes` from `base` on are readable, a lane
+    // past them gets zeros.  Whole K-tiles only in layout K.
+    __device__ __forceinline__ void put(const char* base, uint32_t bytes, char* dst) const {
+#ifdef __HIP_DEVICE_COMPILE__
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, kRsrcFlags);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16, off[i], 0, 0, 0);
+#endif
+    }
     // fragment of the 16 rows from r0, K half s
     static __device__ __forceinline__ typename Frag<T>::type frag(const char* tile, int r0, int s, int lane) {
         if constexpr (!TR) {
@@ -192,8 +206,9 @@ struct GemmArgs {
     int64_t ldc;         // elements
     int batch;           // 2: a.p[1] -> c[1] as a second product of the same shape
     int act;
-    const void* g;       // gated: saved gate and up products (backward: in; forward: out or null)
-    const void* u;
+    float* g;            // gated: saved gate and up products (backward: in; forward: out or null)
+    float* u;
+    int features;        // gated: valid columns; zeros are written past them up to N
     void* h;             // gated forward: h; backward: dg
     void* h2;            // gated backward: du
     int64_t ldh;         // elements, of g, u, h, h2
@@ -234,15 +249,18 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
         if (n < a.N) *reinterpret_cast<f32x4*>(c + n) = acc0;
         if (n2 < a.N) *reinterpret_cast<f32x4*>(c + n2) = acc1;
     } else if constexpr (EPI == kGatedForward) {
-        if (n >= a.N) return;   // N, ldh multiples of 8
+        if (n >= a.N) return;   // N, ldh multiples of 64
         const int64_t o = (int64_t)m * a.ldh + n;
         f32x4 h;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = act_value(a.act, acc0[j]) * acc1[j];
+        for (int j = 0; j < 4; ++j) {
+            if (n + j >= a.features) acc0[j] = acc1[j] = 0.0f;
+            h[j] = act_value(a.act, acc0[j]) * acc1[j];
+        }
         store4((T*)a.h + o, 4, true, h);
         if (a.g) {
-            store4((T*)const_cast<void*>(a.g) + o, 4, true, acc0);
-            store4((T*)const_cast<void*>(a.u) + o, 4, true, acc1);
+            store4(a.g + o, 4, true, acc0);
+            store4(a.u + o, 4, true, acc1);
         }
     } else {
 #pragma unroll
@@ -250,14 +268,14 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
             const int nn = i ? n2 : n;
             if (nn >= a.N) continue;
             const int64_t o = (int64_t)m * a.ldh + nn;
-            const f32x4 g = load4((const T*)a.g + o), u = load4((const T*)a.u + o), dh = i ? acc1 : acc0;
+            const f32x4 g = load4(a.g + o), u = load4(a.u + o), dh = i ? acc1 : acc0;
             f32x4 dg, du;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float v, dv;
                 act_both(a.act, g[j], v, dv);
-                dg[j] = dh[j] * u[j] * dv;
-                du[j] = dh[j] * v;
+                dg[j] = nn + j < a.features ? dh[j] * u[j] * dv : 0.0f;
+                du[j] = nn + j < a.features ? dh[j] * v : 0.0f;
             }
             store4((T*)a.h + o, 4, true, dg);
             store4((T*)a.h2 + o, 4, true, du);
@@ -373,7 +391,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 }
 
 // ---- the tiled product, 256 x 256 -----------------------------------------------------------
-// 16-bit operands, eight waves in 2 (m) x 4 (n), each 2 x 64 rows by 2 x 32 columns: 128
+// 16-bit operands, whole K-tiles where an operand is K-contiguous, eight waves in 2 (m) x 4 (n), each 2 x 64 rows by 2 x 32 columns: 128
 // accumulator registers a lane.  Each operand's tile is two half-tiles of 16 KB; two K-tiles of
 // four half-tiles fill 128 KB of LDS.  A K-tile runs as four phases, one quadrant of the result
 // each (A0 B0, A0 B1, A1 B1, A1 B0; B's halves the other way round in every second K-tile), so a
@@ -432,25 +450,53 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     TB tb;
     ta.init(a.a.ld);
     tb.init(a.b.ld);
-    const int64_t am = TRA ? (int64_t)m0 * 2 : (int64_t)m0 * a.a.ld, ah = TRA ? 256 : 128 * a.a.ld;
-    const int64_t bn = TRB ? (int64_t)n0 * 2 : (int64_t)n0 * a.b.ld, bh = TRB ? 256 : 128 * a.b.ld;
     const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
     const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
-    const char *pa0 = held(a.a.p[a.batch > 1 ? z : 0] + am), *pa1 = held(a.a.p[1] + am);   // a batch has one segment
-    const char *pb0 = held(a.b.p[0] + bn), *pb1 = held(a.b.p[1] + bn);
-    auto stage_a = [&](int h, int kt, int buf) {
-        const bool seg = kt >= nk && a.segments > 1;
-        ta.stage((seg ? pa1 : pa0) + h * ah, a.a.ld, a.a.mn - m0 - h * 128, a.a.k, seg ? kt - nk : kt, smem + buf * BUF + h * HT);
+    // A half-tile's place in its operand, moved on by a K-tile with each load.  Readable bytes:
+    // layout K, the valid rows whole (the K-tile may start anywhere in them, and a row past them
+    // starts past that range); layout T, the K-tile's rows, less in a segment's last one.
+    struct Cursor {
+        const char *p, *second;
+        int64_t step;
+        uint32_t bytes, bytes_last;
     };
-    auto stage_b = [&](int h, int kt, int buf) {
-        char* dst = smem + buf * BUF + (2 + h) * HT;
-        if constexpr (EPI == kGatedForward) {
-            tb.stage(h ? pb1 : pb0, a.b.ld, a.b.mn - n0, a.b.k, kt, dst);
+    auto cursor = [&](const Operand& o, bool tr, const char* p0, const char* p1, int mn, int kvalid) {
+        Cursor c;
+        const int64_t rows = min(mn, 128);
+        c.step = tr ? TA::BK * o.ld : kTileBytes;
+        const int last = kvalid - (nk - 1) * TA::BK;   // layout T: its own k (a padded A may be deeper)
+        if (tr) {
+            c.bytes = mn > 0 ? (uint32_t)((TA::BK - 1) * o.ld + rows * 2) : 0u;
+            c.bytes_last = mn > 0 && last > 0 ? (uint32_t)((last - 1) * o.ld + rows * 2) : 0u;
         } else {
-            const bool seg = kt >= nk && a.segments > 1;
-            tb.stage((seg ? pb1 : pb0) + h * bh, a.b.ld, a.b.mn - n0 - h * 128, a.b.k, seg ? kt - nk : kt, dst);
+            c.bytes = c.bytes_last = mn > 0 ? (uint32_t)((rows - 1) * o.ld + (int64_t)kvalid * 2) : 0u;
         }
+        const int skip = k0 >= nk ? k0 - nk : k0;
+        c.p = (k0 >= nk ? p1 : p0) + skip * c.step;
+        c.second = p1;
+        return c;
     };
+    const int za = a.batch > 1 ? z : 0;   // a batch has one segment
+    const int64_t am = TRA ? (int64_t)m0 * 2 : (int64_t)m0 * a.a.ld, ah = TRA ? 256 : 128 * a.a.ld;
+    const int64_t bn = TRB ? (int64_t)n0 * 2 : (int64_t)n0 * a.b.ld, bh = TRB ? 256 : 128 * a.b.ld;
+    const char *a0 = a.a.p[za] + am, *a1 = a.a.p[1] + am, *b0 = a.b.p[0] + bn, *b1 = a.b.p[1] + bn;
+    Cursor ca[2] = {cursor(a.a, TRA, a0, a1, a.a.mn - m0, a.a.k), cursor(a.a, TRA, a0 + ah, a1 + ah, a.a.mn - m0 - 128, a.a.k)};
+    Cursor cb[2];
+    if constexpr (EPI == kGatedForward) {
+        cb[0] = cursor(a.b, TRB, b0, b0, a.b.mn - n0, a.b.k);
+        cb[1] = cursor(a.b, TRB, b1, b1, a.b.mn - n0, a.b.k);
+    } else {
+        cb[0] = cursor(a.b, TRB, b0, b1, a.b.mn - n0, a.b.k);
+        cb[1] = cursor(a.b, TRB, b0 + bh, b1 + bh, a.b.mn - n0 - 128, a.b.k);
+    }
+    auto advance = [&](const auto& tile, Cursor& c, bool tr, int kt, char* dst) {
+        uint32_t bytes = kt >= total ? 0u : c.bytes;
+        if (tr && (kt == nk - 1 || kt == total - 1)) bytes = c.bytes_last;
+        tile.put(c.p, bytes, dst);
+        c.p = kt == nk - 1 ? c.second : c.p + c.step;
+    };
+    auto stage_a = [&](int h, int kt, int buf) { advance(ta, ca[h], TRA, kt, smem + buf * BUF + h * HT); };
+    auto stage_b = [&](int h, int kt, int buf) { advance(tb, cb[h], TRB, kt, smem + buf * BUF + (2 + h) * HT); };
 
     // layout T: this lane's LDS address of each 16-column block (first k, first half of a K-tile)
     uint32_t pa[4], pb[2];
@@ -506,11 +552,11 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) acc[A][B][t][u] = Frag<T>::mma(fb[B].f[u][s], fa.f[t][s], acc[A][B][t][u]);
+                for (int u = 0; u < 2; ++u) acc[A][B][t][u] = Frag<T>::mma(fb[B].f[u][s], fa.f[t][s], acc[A][B][t][u]);
         __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -600,7 +646,7 @@ template <typename T, bool GATED, int NW>
 __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ x, int64_t ldx, int rows,
                                                           const T* __restrict__ w0, const T* __restrict__ w1,
                                                           int64_t ldw, int K, int N, int act, T* __restrict__ out,
-                                                          int64_t ldo, T* __restrict__ sg, T* __restrict__ su) {
+                                                          int64_t ldo, float* __restrict__ sg, float* __restrict__ su) {
     constexpr int NB = GATED ? 2 : 1, PIECE = 128 / (int)sizeof(T), CH = 16 / (int)sizeof(T);
     constexpr int UNROLL = GATED ? 2 : 4;
     __shared__ f32x4 part[NW][NB][64];
@@ -659,7 +705,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
     }
     if (!live) return;
     const int n = n0 + kc * 4;
-    if constexpr (GATED) {   // ldo a multiple of 8, columns up to it written (zeros past N)
+    if constexpr (GATED) {   // ldo a multiple of 64, columns up to it written (zeros past N)
         f32x4 h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -710,6 +756,7 @@ template <typename T> __global__ __launch_bounds__(256) void ffn_zero_kernel(T* 
 
 // ------------------------------------------------------------------------------------- host
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
+int64_t up64(int64_t x) { return (x + 63) / 64 * 64; }   // a whole 16-bit K-tile
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 size_t esize(int32_t t) { return t == OTF_F32 ? 4 : 2; }
 
@@ -743,7 +790,8 @@ Plan plan_product(const Product& p, int elem) {
         const int64_t m = (a.M + t - 1) / t, n = p.epi == kGatedForward ? (2 * (int64_t)a.N + t - 1) / t : (a.N + t - 1) / t;
         return m * n * a.batch;
     };
-    const int side = elem == 2 && tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
+    const bool whole = (p.tra || a.a.k % 64 == 0) && (p.trb || a.b.k % 64 == 0);
+    const int side = elem == 2 && whole && tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
     int splits = 1;
     if (p.epi == kStore) {
         const int64_t ktiles = (int64_t)(a.a.k + kTileBytes / elem - 1) / (kTileBytes / elem) * a.segments, t = tiles(side);
@@ -790,24 +838,34 @@ hipError_t run_store(const Product& p, float* slab, hipStream_t s) {
 struct Block {
     const otf_ffn_args* o;
     int es;
-    int64_t n, d, f, d8, f8;
-    Operand x{}, wg{}, wu{}, wd{}, dy{};
+    int64_t n, d, f, f64;   // f64: leading dimension of the hidden buffers, zeros past f
+    bool whole;             // operands copied to whole K-tiles (large products of ragged widths)
+    Operand x{}, wg{}, wu{}, wd{}, dy{};   // k: columns there are, zeros past the caller's
     PackArgs pack{};
-    Carver ws;
+    Carver ws{};
 
-    static bool aligned(const void* p, int64_t ld, int64_t cols) {
-        return cols % 8 == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
+    Block(const otf_ffn_args* args, int elem, void* workspace) : o(args), es(elem) {
+        n = o->rows, d = o->d, f = o->f, f64 = up64(f);
+        // ragged widths: a copy costs two passes over the operands, and pays where the products are large
+        whole = es == 2 && ((n + 255) / 256) * ((f + 127) / 128) >= kCus;
+        ws.base = (char*)workspace;
+    }
+
+    bool aligned(const void* p, int64_t ld, int64_t cols) const {
+        return cols % (whole ? 64 : 8) == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
     }
     void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols, bool copy) {
         v.p[0] = v.p[1] = (const char*)p;
         v.ld = ld * es;
+        v.k = (int)cols;
         if (copy) {
-            const int64_t ldd = up8(cols);
+            const int64_t ldd = up64(cols);
             void* dst = ws.take((size_t)(rows * ldd * es));
             pack.item[pack.count++] = PackItem{p, dst, ld, ldd, rows, cols, pack.total};
             pack.total += rows * (ldd / 8);
             v.p[0] = v.p[1] = (const char*)dst;
             v.ld = ldd * es;
+            v.k = (int)ldd;
         }
     }
     void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols) {
@@ -826,10 +884,17 @@ struct Block {
     }
 };
 
-Operand as_operand(const Operand& v, int64_t mn, int64_t k) {
+// an input as layout K (its columns are k, `k` of them) or T (its rows are k)
+Operand by_rows(const Operand& v, int64_t rows, int64_t k) {
     Operand r = v;
-    r.mn = (int)mn;
+    r.mn = (int)rows;
     r.k = (int)k;
+    return r;
+}
+Operand by_columns(const Operand& v, int64_t rows) {
+    Operand r = v;
+    r.mn = v.k;
+    r.k = (int)rows;
     return r;
 }
 Operand buffer_operand(const void* p, int64_t ld, int es, int64_t mn, int64_t k) {
@@ -858,34 +923,33 @@ bool bad_ld(int64_t ld, int64_t cols) { return ld < cols || ld > (1 << 20); }
 bool misaligned(const void* p, int32_t dtype) { return (uintptr_t)p % esize(dtype) != 0; }
 
 struct Saved {
-    char *g, *u, *h;
+    float *g, *u;
+    char* h;
 };
-Saved carve_saved(void* p, int64_t n, int64_t f8, int es) {
-    const size_t one = up256((size_t)(n * f8 * es));
+Saved carve_saved(void* p, int64_t n, int64_t f64, int es) {
     char* b = (char*)p;
-    return Saved{b, b + one, b + 2 * one};
+    const size_t wide = up256((size_t)(n * f64) * 4);
+    return Saved{(float*)b, (float*)(b + wide), b + 2 * wide};
 }
+size_t saved_bytes(int64_t n, int64_t f64, int es) { return 2 * up256((size_t)(n * f64) * 4) + up256((size_t)(n * f64 * es)); }
 
-// forward: returns the workspace it needs in *need; runs where run is set
+// forward: the workspace it needs in *need; runs where run is set
 template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
-    Block b{};
-    b.o = o, b.es = (int)sizeof(T), b.n = o->rows, b.d = o->d, b.f = o->f, b.d8 = up8(o->d), b.f8 = up8(o->f);
-    b.ws.base = (char*)workspace;
-    const bool few = b.n <= kFewRows;
+    Block b(o, (int)sizeof(T), workspace);
     Saved sv{};
     if (o->saved)
-        sv = carve_saved(o->saved, b.n, b.f8, b.es);
+        sv = carve_saved(o->saved, b.n, b.f64, b.es);
     else
-        sv.h = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
-    if (few) {
+        sv.h = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
+    if (b.n <= kFewRows) {
         *need = b.ws.used;
         if (!run) return OTF_OK;
-        const unsigned g1 = (unsigned)((b.f8 + 15) / 16), g2 = (unsigned)((b.d + 15) / 16);
+        const unsigned g1 = (unsigned)(b.f64 / 16), g2 = (unsigned)((b.d + 15) / 16);
         ffn_few_kernel<T, true, 4><<<g1, 256, 0, s>>>((const T*)o->x, o->ldx, (int)b.n, (const T*)o->w_gate,
                                                        (const T*)o->w_up, o->ldw_in, (int)b.d, (int)b.f, o->activation,
-                                                       (T*)sv.h, b.f8, (T*)sv.g, (T*)sv.u);
+                                                       (T*)sv.h, b.f64, sv.g, sv.u);
         OTF_HIP(hipGetLastError());
-        ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.f8, (int)b.n, (const T*)o->w_down, nullptr,
+        ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.f64, (int)b.n, (const T*)o->w_down, nullptr,
                                                         o->ldw_down, (int)b.f, (int)b.d, 0, (T*)o->y, o->ldy, nullptr,
                                                         nullptr);
         return check_hip(hipGetLastError());
@@ -893,10 +957,11 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     b.operand(b.x, o->x, o->ldx, b.n, b.d);
     b.weights_in();
     b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
-    Product in{false, false, kGatedForward, product_args(as_operand(b.x, b.n, b.d8), as_operand(b.wg, b.f, b.d8), b.n, b.f8, nullptr, 0)};
+    const int kin = b.x.k < b.wg.k ? b.x.k : b.wg.k;   // what is copied ends in zeros
+    Product in{false, false, kGatedForward, product_args(by_rows(b.x, b.n, kin), by_rows(b.wg, b.f, kin), b.n, b.f64, nullptr, 0)};
     in.a.b.p[1] = b.wu.p[0];
-    in.a.act = o->activation, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.f8;
-    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.f8, b.es, b.n, b.f8), as_operand(b.wd, b.d, b.f8), b.n, b.d, o->y, o->ldy)};
+    in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.f64;
+    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.f64, b.es, b.n, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
     float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es)));
     *need = b.ws.used;
     if (!run) return OTF_OK;
@@ -907,28 +972,26 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
 }
 
 template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
-    Block b{};
-    b.o = o, b.es = (int)sizeof(T), b.n = o->rows, b.d = o->d, b.f = o->f, b.d8 = up8(o->d), b.f8 = up8(o->f);
-    b.ws.base = (char*)workspace;
-    const Saved sv = carve_saved(o->saved, b.n, b.f8, b.es);
+    Block b(o, (int)sizeof(T), workspace);
+    const Saved sv = carve_saved(o->saved, b.n, b.f64, b.es);
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
-    char* dg = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
-    char* du = (char*)b.ws.take((size_t)(b.n * b.f8 * b.es));
+    char* dg = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
+    char* du = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
     b.operand(b.dy, o->dy, o->lddy, b.n, b.d);
     if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
     if (wx) b.weights_in();
     if (win) b.operand(b.x, o->x, o->ldx, b.n, b.d);
-    // dh = dy Wd: K = d; Wd's rows are k
-    Product mid{false, true, kGatedBackward, product_args(as_operand(b.dy, b.n, b.d8), as_operand(b.wd, b.f8, b.d), b.n, b.f8, nullptr, 0)};
-    mid.a.act = o->activation, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.f8;
-    // dx = dg Wg + du Wu: two segments of K = f
-    Product px{false, true, kStore, product_args(buffer_operand(dg, b.f8, b.es, b.n, b.f8), as_operand(b.wg, b.d8, b.f), b.n, b.d, o->dx, o->lddx)};
+    // dh = dy Wd: K = d, the rows of Wd
+    Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.f64, nullptr, 0)};
+    mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.f64;
+    // dx = dg Wg + du Wu: two segments of K = f, the rows of the weights
+    Product px{false, true, kStore, product_args(buffer_operand(dg, b.f64, b.es, b.n, b.f64), by_columns(b.wg, b.f), b.n, b.d, o->dx, o->lddx)};
     px.a.a.p[1] = du, px.a.b.p[1] = b.wu.p[0], px.a.segments = 2;
     // dWg, dWu = dg^T x, du^T x: a batch of two, K = rows
-    Product pi{true, true, kStore, product_args(buffer_operand(dg, b.f8, b.es, b.f8, b.n), as_operand(b.x, b.d8, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
+    Product pi{true, true, kStore, product_args(buffer_operand(dg, b.f64, b.es, b.f64, b.n), by_columns(b.x, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
     pi.a.a.p[1] = du, pi.a.c[1] = o->dw_up, pi.a.batch = 2;
     // dWd = dy^T h
-    Product pd{true, true, kStore, product_args(as_operand(b.dy, b.d8, b.n), buffer_operand(sv.h, b.f8, b.es, b.f8, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
+    Product pd{true, true, kStore, product_args(by_columns(b.dy, b.n), buffer_operand(sv.h, b.f64, b.es, b.f64, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
     size_t slab = 0;   // one after another on the stream: they share it
     auto more = [&](const Product& p) { const size_t k = slab_bytes(p, plan_product(p, b.es)); slab = k > slab ? k : slab; };
     if (wx) more(px);
@@ -970,7 +1033,7 @@ extern "C" {
 
 size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype) {
     if (rows <= 0 || f <= 0) return 0;
-    return 3 * up256((size_t)(rows * up8(f)) * esize(dtype));
+    return saved_bytes(rows, up64(f), (int)esize(dtype));
 }
 
 size_t otf_gated_ffn_workspace_size(const otf_ffn_args* o) {

@@ -414,7 +414,7 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
     x: (..., d); w_gate, w_up: (f, d); w_down: (d, f), as ``torch.nn.Linear`` keeps them, all of
     x's type.  ``activation``: "silu" or "gelu" (the exact form).  Sums are float32; the hidden
-    activations, and the two products kept for backward, are rounded to x's type."""
+    activations are rounded to x's type, the two products that backward needs are kept in float32."""
     _input(x, "x")
     for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         _input(t, name)
