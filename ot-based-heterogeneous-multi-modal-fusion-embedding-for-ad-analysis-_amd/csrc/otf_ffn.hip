@@ -62,19 +62,38 @@ enum { kSilu = 0, kGelu = 1 };
 __device__ __forceinline__ float sigmoid(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
 }
-__device__ __forceinline__ float act_value(int act, float g) {
-    if (act == kSilu) return g * sigmoid(g);
-    return 0.5f * g * erfcf(-0.70710678118654752f * g);
+// The normal distribution function c(g) and e = exp(-g^2 / 2).  float32 operands: erfc.  16-bit
+// ones: Abramowitz and Stegun 7.1.26, erfc(x) = t (a1 + t (... a5)) exp(-x^2), t = 1 / (1 + p x),
+// within 1.5e-7, which shares the exponential with the derivative (the exact form took 6 us of the
+// 34 of a gate and up product at 777 x 1000 x 2730).
+template <typename T> __device__ __forceinline__ void normal_cdf(float g, float& c, float& e) {
+    const float x = 0.70710678118654752f * fabsf(g);
+    e = __builtin_amdgcn_exp2f(-1.44269504088896341f * x * x);
+    float q;
+    if constexpr (sizeof(T) == 4) {
+        q = erfcf(x);
+    } else {
+        const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * x);
+        q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f)))) * e;
+    }
+    c = g < 0.0f ? 0.5f * q : 1.0f - 0.5f * q;
 }
-__device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
+template <typename T> __device__ __forceinline__ float act_value(int act, float g) {
+    if (act == kSilu) return g * sigmoid(g);
+    float c, e;
+    normal_cdf<T>(g, c, e);
+    return g * c;
+}
+template <typename T> __device__ __forceinline__ void act_both(int act, float g, float& a, float& da) {
     if (act == kSilu) {
         const float s = sigmoid(g);
         a = g * s;
         da = s * (1.0f + g * (1.0f - s));
     } else {
-        const float c = 0.5f * erfcf(-0.70710678118654752f * g);
+        float c, e;
+        normal_cdf<T>(g, c, e);
         a = g * c;
-        da = c + g * 0.39894228040143268f * expf(-0.5f * g * g);
+        da = c + g * 0.39894228040143268f * e;
     }
 }
 
@@ -172,17 +191,8 @@ template <typename T, bool TR, int R, int NT> struct Tile {
             const int row = r0 + (lane & 15);
             return *reinterpret_cast<const typename Frag<T>::type*>(tile + s * (R * 64) + row * 64 +
                                                                     (((lane >> 4) ^ swz_k(row)) << 4));
-        } else if constexpr (sizeof(T) == 2) {
-            const int i = lane & 15, k = s * 32 + (lane >> 4) * 8 + (i >> 2), chunk = r0 / 8 + ((i & 3) >> 1);
-            const char* a = tile + k * (R * 2) + (i & 1) * 8;
-            typename Frag<T>::type f;
-            s16x4* h = reinterpret_cast<s16x4*>(&f);
-            h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(a + ((chunk ^ swz_t<T, R>(k)) << 4)));
-            h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(a + 4 * (R * 2) + ((chunk ^ swz_t<T, R>(k + 4)) << 4)));
-            return f;
         } else {
+            static_assert(sizeof(T) == 4, "16-bit: read_tr");
             typename Frag<T>::type f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -255,7 +265,7 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (n + j >= a.features) acc0[j] = acc1[j] = 0.0f;
-            h[j] = act_value(a.act, acc0[j]) * acc1[j];
+            h[j] = act_value<T>(a.act, acc0[j]) * acc1[j];
         }
         store4((T*)a.h + o, 4, true, h);
         if (a.g) {
@@ -273,7 +283,7 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float v, dv;
-                act_both(a.act, g[j], v, dv);
+                act_both<T>(a.act, g[j], v, dv);
                 dg[j] = nn + j < a.features ? dh[j] * u[j] * dv : 0.0f;
                 du[j] = nn + j < a.features ? dh[j] * v : 0.0f;
             }
@@ -302,16 +312,90 @@ __device__ __forceinline__ const char* held(const char* p) {
     return p;
 }
 
+// N fragments of layout T over a whole K-tile: f[block][half of K][four k], from this lane's
+// addresses of the blocks' first k, rows of ROW bytes (the permutation of a row's chunks is the
+// same four rows on and half a K-tile on).  In assembly because the compiler waits for every load
+// in flight before such a read; the wait for the reads is part of the block, so nothing after it
+// can use a register whose read is under way.
+template <int N, int ROW, int OFF> __device__ __forceinline__ void read_tr(const uint32_t (&p)[N], s16x4 (&f)[N][2][2]) {
+    static_assert(N == 1 || N == 2 || N == 4, "blocks");
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (N == 1)
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %4 offset:%5\n\t"
+            "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+            "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+            "ds_read_b64_tr_b16 %3, %4 offset:%8\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1])
+            : "v"(p[0]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
+            : "memory");
+    if constexpr (N == 2)
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
+            "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
+            "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
+            "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
+            "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]), "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1])
+            : "v"(p[0]), "v"(p[1]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
+            : "memory");
+    if constexpr (N == 4)
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %16 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
+            "ds_read_b64_tr_b16 %2, %16 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %3, %16 offset:%23\n\t"
+            "ds_read_b64_tr_b16 %4, %17 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %5, %17 offset:%21\n\t"
+            "ds_read_b64_tr_b16 %6, %17 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %7, %17 offset:%23\n\t"
+            "ds_read_b64_tr_b16 %8, %18 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %9, %18 offset:%21\n\t"
+            "ds_read_b64_tr_b16 %10, %18 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %11, %18 offset:%23\n\t"
+            "ds_read_b64_tr_b16 %12, %19 offset:%20\n\t"
+            "ds_read_b64_tr_b16 %13, %19 offset:%21\n\t"
+            "ds_read_b64_tr_b16 %14, %19 offset:%22\n\t"
+            "ds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]), "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1]), "=&v"(f[2][0][0]), "=&v"(f[2][0][1]), "=&v"(f[2][1][0]), "=&v"(f[2][1][1]), "=&v"(f[3][0][0]), "=&v"(f[3][0][1]), "=&v"(f[3][1][0]), "=&v"(f[3][1][1])
+            : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
+            : "memory");
+#endif
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// N fragments of a tile, both halves of K, in either layout
+template <typename T, int N> union Frags {
+    s16x4 h[N][2][2];
+    typename Frag<T>::type f[N][2];
+    __device__ __forceinline__ Frags() {}
+};
+// this lane's LDS address of the block of 16 columns from r0 in a layout T tile of R columns
+template <typename T, int R> __device__ __forceinline__ uint32_t tr_address(const char* tile, int r0, int lane) {
+    const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)tile + k * (R * 2) +
+           (((r0 / 8 + ((i & 3) >> 1)) ^ swz_t<T, R>(k)) << 4) + (i & 1) * 8;
+}
+
 // ---- the tiled product -----------------------------------------------------------------
-// TM x TN tile (B in two halves of TN / 2), WGM x WGN waves; K-tiles double-buffered: the
-// next one is on its way while this one's MFMAs run, one barrier a K-tile.
-template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int EPI>
+// TM x TN tile (B in two halves of TN / 2), WGM x WGN waves.  S buffers of one K-tile: S - 1 are on
+// their way while the MFMAs of one run, one barrier a K-tile.  These tiles serve products that do
+// not fill the chip with large ones, whose K loop is bound by the latency of a load.
+template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int S, int EPI>
 __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
     constexpr int NT = 64 * WGM * WGN, TH = TN / 2, RA = TM / WGM / 16, RB = TH / WGN / 16;
     using TA = Tile<T, TRA, TM, NT>;
     using TB = Tile<T, TRB, TH, NT>;
     constexpr int BUF = TA::BYTES + 2 * TB::BYTES;
-    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
+    constexpr int LOADS = TA::PER + 2 * TB::PER;   // a wave's, a K-tile
+    static_assert(TA::CHUNKS % NT == 0 && TB::CHUNKS % NT == 0, "every wave issues the same loads");
+    __shared__ __attribute__((aligned(16))) char smem[S * BUF];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / WGN, wn = wid % WGN;
 
     const int tiles = a.tiles_m * a.tiles_n, z = blockIdx.y % a.batch, split = blockIdx.y / a.batch;
@@ -332,7 +416,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
     const char *pa0 = held(a.a.p[a.batch > 1 ? z : 0] + am), *pa1 = held(a.a.p[1] + am);   // a batch has one segment
     const char *pb0 = held(a.b.p[0] + bn), *pb1 = held(a.b.p[1] + bn);
     auto stage = [&](int kt, int buf) {
-        const int seg = kt >= nk ? 1 : 0, k = kt - seg * nk;
+        const int seg = a.segments > 1 && kt >= nk ? 1 : 0, k = kt - seg * nk;
         char* dst = smem + buf * BUF;
         ta.stage(seg ? pa1 : pa0, a.a.ld, a.a.mn - m0, a.a.k, k, dst);
         const char* b0 = EPI != kGatedForward && seg ? pb1 : pb0;
@@ -349,28 +433,55 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
             for (int i = 0; i < RA; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    if (k0 < k1) stage(k0, 0);
+    uint32_t xa[RA], xb[RB];   // layout T: addresses in the first buffer
+#pragma unroll
+    for (int i = 0; i < RA; ++i) xa[i] = tr_address<T, TM>(smem, (wm * RA + i) * 16, lane);
+#pragma unroll
+    for (int j = 0; j < RB; ++j) xb[j] = tr_address<T, TH>(smem + TA::BYTES, (wn * RB + j) * 16, lane);
+
+    // past the end of K (k1: past this split's) the loads bring what nothing reads; the counts hold
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) stage(k0 + i, i);
+    int buf = 0;
     for (int kt = k0; kt < k1; ++kt) {
-        const int buf = (kt - k0) & 1;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+        wait_loads<(S - 2) * LOADS>();
+        __builtin_amdgcn_s_barrier();   // K-tile kt is there for every wave, and kt - 1 read by all
         asm volatile("" ::: "memory");
-        // every fragment of the K-tile first, then the next tile's loads: the compiler waits
-        // for loads in flight before a transposed LDS read, so none may be
+        const int next = buf == 0 ? S - 1 : buf - 1;
         const char* sa = smem + buf * BUF;
         const char* sb = sa + TA::BYTES;
-        typename Frag<T>::type fa[2][RA], fb[2][2][RB];
+        Frags<T, RA> fa;
+        Frags<T, RB> fb[2];
+        if constexpr ((TRA || TRB) && sizeof(T) == 2) stage(kt + S - 1, next);
+        if constexpr (TRA && sizeof(T) == 2) {
+            uint32_t p[RA];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
+            for (int i = 0; i < RA; ++i) p[i] = xa[i] + buf * BUF;
+            read_tr<RA, TM * 2, 0>(p, fa.h);
+        } else {
 #pragma unroll
-            for (int i = 0; i < RA; ++i) fa[s][i] = TA::frag(sa, (wm * RA + i) * 16, s, lane);
+            for (int i = 0; i < RA; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) fa.f[i][s] = TA::frag(sa, (wm * RA + i) * 16, s, lane);
+        }
+        if constexpr (TRB && sizeof(T) == 2) {
+            uint32_t p[RB];
+#pragma unroll
+            for (int j = 0; j < RB; ++j) p[j] = xb[j] + buf * BUF;
+            read_tr<RB, TH * 2, 0>(p, fb[0].h);
+            read_tr<RB, TH * 2, TB::BYTES>(p, fb[1].h);
+        } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < RB; ++j) fb[s][h][j] = TB::frag(sb + h * TB::BYTES, (wn * RB + j) * 16, s, lane);
+                for (int j = 0; j < RB; ++j)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) fb[h].f[j][s] = TB::frag(sb + h * TB::BYTES, (wn * RB + j) * 16, s, lane);
         }
-        asm volatile("" ::: "memory");
-        if (kt + 1 < k1) stage(kt + 1, buf ^ 1);
+        if constexpr (!((TRA || TRB) && sizeof(T) == 2)) {
+            asm volatile("" ::: "memory");
+            stage(kt + S - 1, next);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -378,8 +489,11 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
                 for (int j = 0; j < RB; ++j)
 #pragma unroll
-                    for (int i = 0; i < RA; ++i) acc[h][j][i] = Frag<T>::mma(fb[s][h][j], fa[s][i], acc[h][j][i]);
+                    for (int i = 0; i < RA; ++i) acc[h][j][i] = Frag<T>::mma(fb[h].f[j][s], fa.f[i][s], acc[h][j][i]);
+        // the reads have returned (the MFMAs used them) before this wave reaches the next barrier
+        buf = buf + 1 == S ? 0 : buf + 1;
     }
+    wait_loads<0>();
     // B is the first operand of the MFMAs, so a lane holds four consecutive n of one m
 #pragma unroll
     for (int i = 0; i < RA; ++i)
@@ -398,46 +512,12 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 // phase reads only the fragments that the registers do not hold, 8, 4, 8 and 4 of them.  Each
 // phase puts one half-tile in flight, up to two K-tiles ahead.  The two wave groups (m) run one
 // barrier apart, so on every SIMD one wave's MFMAs cover the other's LDS reads and loads.
-template <int OFF> __device__ __forceinline__ void read_tr4(const uint32_t (&p)[4], s16x4 (&f)[4][2][2]) {
-    // the wait is part of the block: nothing after it can use a register whose read is under way
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %16 offset:%20\n\tds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
-        "ds_read_b64_tr_b16 %2, %16 offset:%22\n\tds_read_b64_tr_b16 %3, %16 offset:%23\n\t"
-        "ds_read_b64_tr_b16 %4, %17 offset:%20\n\tds_read_b64_tr_b16 %5, %17 offset:%21\n\t"
-        "ds_read_b64_tr_b16 %6, %17 offset:%22\n\tds_read_b64_tr_b16 %7, %17 offset:%23\n\t"
-        "ds_read_b64_tr_b16 %8, %18 offset:%20\n\tds_read_b64_tr_b16 %9, %18 offset:%21\n\t"
-        "ds_read_b64_tr_b16 %10, %18 offset:%22\n\tds_read_b64_tr_b16 %11, %18 offset:%23\n\t"
-        "ds_read_b64_tr_b16 %12, %19 offset:%20\n\tds_read_b64_tr_b16 %13, %19 offset:%21\n\t"
-        "ds_read_b64_tr_b16 %14, %19 offset:%22\n\tds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]),
-          "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1]), "=&v"(f[2][0][0]), "=&v"(f[2][0][1]),
-          "=&v"(f[2][1][0]), "=&v"(f[2][1][1]), "=&v"(f[3][0][0]), "=&v"(f[3][0][1]), "=&v"(f[3][1][0]),
-          "=&v"(f[3][1][1])
-        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF), "n"(OFF + 1024), "n"(OFF + 8192), "n"(OFF + 9216)
-        : "memory");
-}
-template <int OFF> __device__ __forceinline__ void read_tr2(const uint32_t (&p)[2], s16x4 (&f)[2][2][2]) {
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8 offset:%10\n\tds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
-        "ds_read_b64_tr_b16 %2, %8 offset:%12\n\tds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %4, %9 offset:%10\n\tds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
-        "ds_read_b64_tr_b16 %6, %9 offset:%12\n\tds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]),
-          "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1])
-        : "v"(p[0]), "v"(p[1]), "n"(OFF), "n"(OFF + 1024), "n"(OFF + 8192), "n"(OFF + 9216)
-        : "memory");
-}
-template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
-
 template <typename T, bool TRA, bool TRB, int EPI>
 __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     static_assert(sizeof(T) == 2, "16-bit operands");
     constexpr int HT = 128 * kTileBytes, BUF = 4 * HT;   // half-tiles A0, A1, B0, B1
     using TA = Tile<T, TRA, 128, 512>;
     using TB = Tile<T, TRB, 128, 512>;
-    using F = typename Frag<T>::type;
     __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid >> 2, wn = wid & 3;
 
@@ -498,32 +578,18 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     auto stage_a = [&](int h, int kt, int buf) { advance(ta, ca[h], TRA, kt, smem + buf * BUF + h * HT); };
     auto stage_b = [&](int h, int kt, int buf) { advance(tb, cb[h], TRB, kt, smem + buf * BUF + (2 + h) * HT); };
 
-    // layout T: this lane's LDS address of each 16-column block (first k, first half of a K-tile)
-    uint32_t pa[4], pb[2];
-    {
-        const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
-        const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-        auto at = [&](int r0) {
-            return base + k * 256 + (((r0 / 8 + ((i & 3) >> 1)) ^ swz_t<T, 128>(k)) << 4) + (i & 1) * 8;
-        };
+    uint32_t xa[4], xb[2];   // layout T: addresses in the first buffer
 #pragma unroll
-        for (int t = 0; t < 4; ++t) pa[t] = at(wm * 64 + t * 16);
+    for (int t = 0; t < 4; ++t) xa[t] = tr_address<T, 128>(smem, wm * 64 + t * 16, lane);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) pb[u] = at(wn * 32 + u * 16);
-    }
-    union FA {
-        s16x4 h[4][2][2];
-        F f[4][2];
-    } fa;
-    union FB {
-        s16x4 h[2][2][2];
-        F f[2][2];
-    } fb[2];
+    for (int u = 0; u < 2; ++u) xb[u] = tr_address<T, 128>(smem, wn * 32 + u * 16, lane);
+    Frags<T, 4> fa;
+    Frags<T, 2> fb[2];
     auto read_a = [&](int buf, auto half) {
         constexpr int H = decltype(half)::value;
         if constexpr (TRA) {
-            const uint32_t p[4] = {pa[0] + buf * BUF, pa[1] + buf * BUF, pa[2] + buf * BUF, pa[3] + buf * BUF};
-            read_tr4<H * HT>(p, fa.h);
+            const uint32_t p[4] = {xa[0] + buf * BUF, xa[1] + buf * BUF, xa[2] + buf * BUF, xa[3] + buf * BUF};
+            read_tr<4, 256, H * HT>(p, fa.h);
         } else {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -534,8 +600,8 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     auto read_b = [&](int buf, auto half) {
         constexpr int H = decltype(half)::value;
         if constexpr (TRB) {
-            const uint32_t p[2] = {pb[0] + buf * BUF, pb[1] + buf * BUF};
-            read_tr2<(2 + H) * HT>(p, fb[H].h);
+            const uint32_t p[2] = {xb[0] + buf * BUF, xb[1] + buf * BUF};
+            read_tr<2, 256, (2 + H) * HT>(p, fb[H].h);
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -710,7 +776,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (n + j >= N) s[0][j] = s[1][j] = 0.0f;
-            h[j] = act_value(act, s[0][j]) * s[1][j];
+            h[j] = act_value<T>(act, s[0][j]) * s[1][j];
         }
         if (n >= ldo) return;
         const int64_t o = (int64_t)r * ldo + n;
@@ -813,9 +879,9 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     if (q.tm == 256) {
         if constexpr (sizeof(T) == 2) ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
     } else if (q.tm == 128)
-        ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
+        ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
     else
-        ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
+        ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
 

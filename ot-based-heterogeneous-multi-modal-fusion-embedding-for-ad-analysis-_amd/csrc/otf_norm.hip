@@ -303,17 +303,36 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     const float inv = 1.0f / (float)cols;
     DropKey key{};
     if constexpr (DROP) key = drop_key(a.rng);
-    for (int64_t row = (int64_t)blockIdx.x * RPB + part; row < a.rows; row += (int64_t)gridDim.x * RPB) {
+    // where the registers allow, the next row is on its way while this one is reduced and stored:
+    // a workgroup has one row at a time, and its loads' latency would stand between rows
+    // (16384 x 4096 bf16: 131 us without)
+    constexpr bool AHEAD = CH * (sizeof(T) + sizeof(TR)) <= 16;
+    typename Chunk8<TR>::type rx[CH];
+    typename Chunk8<T>::type rg[CH];
+    float row_mean = 0.0f, row_rstd = 0.0f;
+    auto fetch = [&](int64_t row) {
         const TR* x = (const TR*)a.x + row * a.ldx;
         const T* dy = (const T*)a.dy + row * a.lddy;
-        float v[CH][8], g[CH][8];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int col = (c * TPR + t) * 8;
-            load8(x + col, cols - col, v[c]);
-            load8(dy + col, cols - col, g[c]);
+            rx[c] = load8_raw(x + col, cols - col);
+            rg[c] = load8_raw(dy + col, cols - col);
         }
-        const float mean = a.mean[row], rstd = a.rstd[row];
+        row_mean = a.mean[row];
+        row_rstd = a.rstd[row];
+    };
+    const int64_t first = (int64_t)blockIdx.x * RPB + part, step = (int64_t)gridDim.x * RPB;
+    if (AHEAD && first < a.rows) fetch(first);
+    for (int64_t row = first; row < a.rows; row += step) {
+        if (!AHEAD) fetch(row);
+        float v[CH][8], g[CH][8];
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[c][j] = (float)rx[c][j], g[c][j] = (float)rg[c][j];
+        const float mean = row_mean, rstd = row_rstd;
+        if (AHEAD && row + step < a.rows) fetch(row + step);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {

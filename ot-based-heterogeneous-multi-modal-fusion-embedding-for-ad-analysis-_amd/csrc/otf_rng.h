@@ -71,6 +71,19 @@ template <typename T> struct Chunk8 {
     using type = T __attribute__((ext_vector_type(8), aligned(sizeof(T))));
 };
 
+// as stored, zeros past `valid`
+template <typename T> __device__ __forceinline__ typename Chunk8<T>::type load8_raw(const T* p, int valid) {
+    typename Chunk8<T>::type q{};
+    if (valid >= 8) {
+        q = *reinterpret_cast<const typename Chunk8<T>::type*>(p);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < valid) q[j] = p[j];
+    }
+    return q;
+}
+
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int valid, float (&v)[8]) {
     if (valid >= 8) {

@@ -241,4 +241,6 @@ def ptr(t) -> int | None:
 
 
 def stream_handle(device=None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of `device` (a torch.device with an index, or None: the current one)."""
+    index = getattr(device, "index", None)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
