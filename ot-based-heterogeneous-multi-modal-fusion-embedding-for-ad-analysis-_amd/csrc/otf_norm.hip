@@ -22,7 +22,9 @@
 namespace otf {
 namespace {
 
-constexpr int kMaxHeldCols = 32768;   // 1024 threads x 4 chunks of 8
+// widest rows held in registers: 1024 threads x 4 chunks of 8; backward, which also holds the
+// parameter gradients' sums, 512 threads x 4
+constexpr int kMaxHeldCols = 32768, kMaxHeldColsBackward = 16384;
 
 struct NormArgs {
     const void* x;       // forward: input; backward: the normalised input (x or z)
@@ -306,7 +308,7 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     // where the registers allow, the next row is on its way while this one is reduced and stored:
     // a workgroup has one row at a time, and its loads' latency would stand between rows
     // (16384 x 4096 bf16: 131 us without)
-    constexpr bool AHEAD = CH * (sizeof(T) + sizeof(TR)) <= 16;
+    constexpr bool AHEAD = NT == 256 && CH * (sizeof(T) + sizeof(TR)) <= 16;
     typename Chunk8<TR>::type rx[CH];
     typename Chunk8<T>::type rg[CH];
     float row_mean = 0.0f, row_rstd = 0.0f;
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     }
 }
 
-// Rows wider than kMaxHeldCols: dx (and dresidual) by one workgroup a row.
+// Rows wider than kMaxHeldColsBackward: dx (and dresidual) by one workgroup a row.
 template <typename T, typename TR, bool DROP>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
     __shared__ float red[2 * 16 * 2];
@@ -452,8 +454,8 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
     }
 }
 
-// Parameter gradients of rows wider than kMaxHeldCols: 64 chunks of 8 columns by 4 waves,
-// each wave every fourth row.
+// Parameter gradients of rows wider than kMaxHeldColsBackward: 64 chunks of 8 columns by 4 waves;
+// the rows are dealt to gridDim.y workgroups and their waves in turn, one partial a workgroup.
 template <typename T, typename TR>
 __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
     __shared__ float comb[3 * 64 * 16];
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[0][j] = 0.0f, s[1][j] = 0.0f;
     if (valid > 0)
-        for (int64_t row = part; row < a.rows; row += 4) {
+        for (int64_t row = (int64_t)blockIdx.y * 4 + part; row < a.rows; row += (int64_t)gridDim.y * 4) {
             const float mean = a.mean[row], rstd = a.rstd[row];
             float v[8], g[8];
             load8((const TR*)a.x + row * a.ldx + col, valid, v);
@@ -484,14 +486,7 @@ __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i >> 3][i & 7] += comb[(p * 16 + i) * 64 + t];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        void* out = i ? a.db : a.dw;
-        if (!out) continue;
-        if (a.wf32)
-            store8((float*)out + col, valid, s[i]);
-        else
-            store8((T*)out + col, valid, s[i]);
-    }
+    for (int i = 0; i < 2; ++i) store8(a.partial + ((int64_t)blockIdx.y * 2 + i) * a.cols + col, valid, s[i]);
 }
 
 // partial [groups][2][cols] -> dw (blockIdx.y = 0), db (1).  64 columns a workgroup, its 16
@@ -546,40 +541,40 @@ hipError_t norm_forward(const NormArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// Workgroups of the backward pass, each of which leaves one partial of dw and db.
+// Workgroups of the backward pass, each of which leaves one partial of dw and db.  Up to 2048
+// columns a workgroup's row is short and its latency bounds: 1024 of them (4099 x 1531 float16: 27
+// -> 25 us), until the partials' traffic counts (16384 x 2048 float32: 88 us, 82 with 512).
 int norm_backward_groups(int64_t rows, int64_t cols) {
-    if (cols > kMaxHeldCols) return 1;
-    const int64_t per = cols <= 2048 ? 4 : 1;
-    const int64_t want = (rows + per - 1) / per, most = cols <= 8192 ? 512 : 256;
+    const bool held = cols <= kMaxHeldColsBackward;
+    const int64_t per = !held ? 64 : cols <= 1024 ? 4 : 1;
+    const int64_t most = !held ? 32 : cols > 8192 ? 256 : cols > 1024 && cols <= 2048 && rows < 8192 ? 1024 : 512;
+    const int64_t want = (rows + per - 1) / per;
     return (int)(want < most ? want : most);
 }
 
 template <typename T, typename TR, bool DROP, bool WG>
 hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
-    const int c = a.cols;
-    if (c > kMaxHeldCols) {
-        norm_backward_long_kernel<T, TR, DROP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
-        if (WG) norm_param_long_kernel<T, TR><<<(unsigned)((c - 1) / 512 + 1), 256, 0, s>>>(a);
-        return hipGetLastError();
-    }
-    const int grid = norm_backward_groups(a.rows, c);
+    const int c = a.cols, grid = norm_backward_groups(a.rows, c);
+    const bool held = c <= kMaxHeldColsBackward;
 #define OTF_NB(NT, TPR, CH) norm_backward_kernel<T, TR, DROP, WG, NT, TPR, CH><<<grid, NT, 0, s>>>(a)
-    if (c <= 512)
+    if (c <= 512) {
         OTF_NB(256, 64, 1);
-    else if (c <= 1024)
+    } else if (c <= 1024) {
         OTF_NB(256, 64, 2);
-    else if (c <= 2048)
-        OTF_NB(256, 64, 4);
-    else if (c <= 4096)
+    } else if (c <= 2048) {
+        OTF_NB(256, 256, 1);
+    } else if (c <= 4096) {
         OTF_NB(256, 256, 2);
-    else if (c <= 8192)
+    } else if (c <= 8192) {
         OTF_NB(256, 256, 4);
-    else if (c <= 16384)
-        OTF_NB(1024, 1024, 2);
-    else
-        OTF_NB(1024, 1024, 4);
+    } else if (held) {
+        OTF_NB(512, 512, 4);
+    } else {
+        norm_backward_long_kernel<T, TR, DROP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+        if (WG) norm_param_long_kernel<T, TR><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
+    }
 #undef OTF_NB
-    if (WG && grid > 1) {
+    if (WG && (grid > 1 || !held)) {
         const dim3 g((unsigned)((c + 63) / 64), 2);
         if (a.wf32)
             norm_param_kernel<float><<<g, 1024, 0, s>>>(a.partial, grid, c, (float*)a.dw, (float*)a.db);
@@ -715,9 +710,9 @@ int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const 
 }
 
 size_t otf_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
-    if (rows <= 0 || cols <= 0 || cols > kMaxHeldCols) return 0;
+    if (rows <= 0 || cols <= 0) return 0;
     const int g = norm_backward_groups(rows, cols);
-    return g > 1 ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;
+    return g > 1 || cols > kMaxHeldColsBackward ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;
 }
 
 // shared by the two backward entry points
