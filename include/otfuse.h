@@ -636,20 +636,22 @@ int otf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
                             int64_t cols, void* dx, int64_t lddx, void* dweight, void* dbias, void* workspace,
                             size_t workspace_bytes, otf_stream_t stream);
 
-/* z = residual + dropout(x) (rdtype: dtype or OTF_F32; rounded once), y = layer norm of z as
- * stored.  residual, z: rdtype; x, y: dtype.                                               */
+/* z = residual + dropout(x), y = layer norm of the float32 sum; each rounded once.
+ * residual, z: rdtype (dtype or OTF_F32); x, y: dtype.                                     */
 int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const void* residual, int64_t ldr,
                                int32_t rdtype, const void* weight, const void* bias, int32_t wdtype, double eps,
                                double p, const int64_t* rng, int64_t rows, int64_t cols, void* y, int64_t ldy,
                                void* z, int64_t ldz, float* mean, float* rstd, otf_stream_t stream);
 
 /* From dy (of y) and dz (of z, NULL: zero): dresidual = dz + LN'(dy), dx = dropout'(dresidual),
- * dweight, dbias.  Workspace: otf_layer_norm_backward_workspace_size.                       */
+ * dweight, dbias.  Reads z where rdtype is OTF_F32 (x, residual unused), else the forward's x and
+ * residual (z unused).  Workspace: otf_layer_norm_backward_workspace_size.                  */
 int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void* dz, int64_t lddz, const void* z,
-                                        int64_t ldz, int32_t dtype, int32_t rdtype, const void* weight,
-                                        int32_t wdtype, const float* mean, const float* rstd, double p,
-                                        const int64_t* rng, int64_t rows, int64_t cols, void* dx, int64_t lddx,
-                                        void* dresidual, int64_t lddr, void* dweight, void* dbias, void* workspace,
+                                        int64_t ldz, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                        int32_t dtype, int32_t rdtype, const void* weight, int32_t wdtype,
+                                        const float* mean, const float* rstd, double p, const int64_t* rng,
+                                        int64_t rows, int64_t cols, void* dx, int64_t lddx, void* dresidual,
+                                        int64_t lddr, void* dweight, void* dbias, void* workspace,
                                         size_t workspace_bytes, otf_stream_t stream);
 
 /* ------------------------------------------------------------------------------------

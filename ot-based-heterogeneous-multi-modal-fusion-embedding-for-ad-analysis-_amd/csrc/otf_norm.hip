@@ -10,9 +10,11 @@
 //                          E[x^2] - mean^2 would cancel for rows with a large mean)
 //   its backward           c = dy w;  dx = rstd (c - mean(c) - xhat mean(c xhat));
 //                          dw = sum_rows dy xhat;  db = sum_rows dy
-//   residual norm          z = residual + dropout(x), y = LN(z), of z as it is stored, so
-//                          backward, which reads z, sees the same row; backward adds the
-//                          gradient that reaches z directly
+//   residual norm          z = residual + dropout(x), y = LN(z) of the float32 sum; backward adds
+//                          the gradient that reaches z directly.  It reads z where z is stored
+//                          in float32 and makes the sum again from x and residual where z was
+//                          rounded to 16 bits: dw sums dy xhat over the rows, which a rounded
+//                          row would put off by 2e-3 (2 more bytes an element, of 10)
 //
 // dw and db: every workgroup keeps float32 partials of its rows in registers and writes them
 // once; a second launch adds the partials in a fixed order (no atomics: the same bits every
@@ -27,10 +29,12 @@ namespace {
 constexpr int kMaxHeldCols = 32768, kMaxHeldColsBackward = 16384;
 
 struct NormArgs {
-    const void* x;       // forward: input; backward: the normalised input (x or z)
+    const void* x;       // forward: input; backward: the normalised input (x or z), or with res x
     int64_t ldx;
-    const void* res;     // forward: residual; backward: dz (may be null)
+    const void* res;     // residual
     int64_t ldr;
+    const void* dz;      // backward (may be null)
+    int64_t lddz;
     const void* dy;      // backward
     int64_t lddy;
     void* y;             // forward: y; backward: dx
@@ -116,7 +120,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, i
     load8(x + ox, valid, v);
     float r[8];
     if constexpr (RES) load8(res + orr, valid, r);
-    drop8(v, g, drop_key(rng), threshold, scale);
+    drop8(v, keep8(g, drop_key(rng), threshold), scale);
     if constexpr (RES)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += r[j];
@@ -153,9 +157,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_forward_kernel(Nor
             if (col >= cols) continue;
             float r[8];
             load8(res + col, cols - col, r);
-            drop8(v[c], first + (uint32_t)(col / 8), key, a.threshold, a.scale);
+            drop8(v[c], keep8(first + (uint32_t)(col / 8), key, a.threshold), a.scale);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[c][j] = col + j < cols ? (float)(TR)(v[c][j] + r[j]) : 0.0f;
+            for (int j = 0; j < 8; ++j) v[c][j] = col + j < cols ? v[c][j] + r[j] : 0.0f;
             store8(z + col, cols - col, v[c]);
         }
     }
@@ -210,30 +214,33 @@ __global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormArgs a) {
     const T* x = (const T*)a.x + row * a.ldx;
     TR* z = DROP ? (TR*)a.z + row * a.ldz : nullptr;
     float s[1] = {0.0f};
-    for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
-        const int valid = (int)(cols - col < 8 ? cols - col : 8);
-        float v[8];
+    auto sum_of = [&](int64_t col, int valid, float (&v)[8]) {   // the row's values, in float32
         load8(x + col, valid, v);
         if constexpr (DROP) {
             float r[8];
             load8((const TR*)a.res + row * a.ldr + col, valid, r);
-            drop8(v, (uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng), a.threshold,
-                  a.scale);
+            const uint64_t index = (uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8);
+            drop8(v, keep8(index, drop_key(a.rng), a.threshold), a.scale);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = j < valid ? (float)(TR)(v[j] + r[j]) : 0.0f;
-            store8(z + col, valid, v);
+            for (int j = 0; j < 8; ++j) v[j] = j < valid ? v[j] + r[j] : 0.0f;
         }
+    };
+    for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
+        const int valid = (int)(cols - col < 8 ? cols - col : 8);
+        float v[8];
+        sum_of(col, valid, v);
+        if constexpr (DROP) store8(z + col, valid, v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[0] += v[j];
     }
     row_sums<1024, 1>(s, red, gen);
     const float mean = s[0] / (float)cols;
     s[0] = 0.0f;
-    auto again = [&](int64_t col, int valid, float (&v)[8]) {   // this thread's own z, or x
-        if constexpr (DROP)
+    auto again = [&](int64_t col, int valid, float (&v)[8]) {   // this thread's own z where it holds the sum
+        if constexpr (DROP && sizeof(TR) == 4)
             load8((const TR*)z + col, valid, v);
         else
-            load8(x + col, valid, v);
+            sum_of(col, valid, v);
     };
     for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
         const int valid = (int)(cols - col < 8 ? cols - col : 8);
@@ -284,8 +291,8 @@ __device__ __forceinline__ void store_param_grad(const NormArgs& a, int which, i
     }
 }
 
-// Rows gridDim RPB apart.  WG: parameter gradients wanted.  TR: the type of z (= T without
-// the residual sum).
+// Rows gridDim RPB apart.  WG: parameter gradients wanted.  TR: the type of residual and z (= T
+// without the residual sum); a 16-bit one makes the sum again from x and residual.
 template <typename T, typename TR, bool DROP, bool WG, int NT, int TPR, int CH>
 __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     constexpr int RPB = NT / TPR;
@@ -308,8 +315,9 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     // where the registers allow, the next row is on its way while this one is reduced and stored:
     // a workgroup has one row at a time, and its loads' latency would stand between rows
     // (16384 x 4096 bf16: 131 us without)
-    constexpr bool AHEAD = NT == 256 && CH * (sizeof(T) + sizeof(TR)) <= 16;
-    typename Chunk8<TR>::type rx[CH];
+    constexpr bool AGAIN = DROP && sizeof(TR) == 2;
+    constexpr bool AHEAD = NT == 256 && CH * (sizeof(T) + sizeof(TR) + (AGAIN ? 2 : 0)) <= 16;
+    typename Chunk8<TR>::type rx[CH], rr[CH];
     typename Chunk8<T>::type rg[CH];
     float row_mean = 0.0f, row_rstd = 0.0f;
     auto fetch = [&](int64_t row) {
@@ -320,6 +328,7 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
             const int col = (c * TPR + t) * 8;
             rx[c] = load8_raw(x + col, cols - col);
             rg[c] = load8_raw(dy + col, cols - col);
+            if constexpr (AGAIN) rr[c] = load8_raw((const TR*)a.res + row * a.ldr + col, cols - col);
         }
         row_mean = a.mean[row];
         row_rstd = a.rstd[row];
@@ -329,10 +338,19 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     for (int64_t row = first; row < a.rows; row += step) {
         if (!AHEAD) fetch(row);
         float v[CH][8], g[CH][8];
+        uint32_t kept[CH];
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[c][j] = (float)rx[c][j], g[c][j] = (float)rg[c][j];
+            if constexpr (DROP)
+                kept[c] = keep8((uint64_t)row * (uint32_t)((cols + 7) / 8) + (uint32_t)(c * TPR + t), key, a.threshold);
+            if constexpr (AGAIN) {
+                drop8(v[c], kept[c], a.scale);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[c][j] += (float)rr[c][j];
+            }
+        }
         const float mean = row_mean, rstd = row_rstd;
         if (AHEAD && row + step < a.rows) fetch(row + step);
         float s[2] = {0.0f, 0.0f};
@@ -361,14 +379,14 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[c][j] = rstd * (g[c][j] - m1 - v[c][j] * m2);
             if constexpr (DROP) {
-                if (a.res) {
+                if (a.dz) {
                     float r[8];
-                    load8((const TR*)a.res + row * a.ldr + col, cols - col, r);
+                    load8((const TR*)a.dz + row * a.lddz + col, cols - col, r);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) g[c][j] += r[j];
                 }
                 store8((TR*)a.z + row * a.ldz + col, cols - col, g[c]);
-                drop8(g[c], (uint64_t)row * (uint32_t)((cols + 7) / 8) + (uint32_t)(col / 8), key, a.threshold, a.scale);
+                drop8(g[c], kept[c], a.scale);
             }
             store8((T*)a.y + row * a.ldy + col, cols - col, g[c]);
         }
@@ -403,6 +421,17 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     }
 }
 
+// x -> residual + dropout(x) of one chunk
+template <typename TR>
+__device__ __forceinline__ void add_residual(const NormArgs& a, int64_t row, int64_t col, int valid, uint32_t kept,
+                                             float (&v)[8]) {
+    float r[8];
+    load8((const TR*)a.res + row * a.ldr + col, valid, r);
+    drop8(v, kept, a.scale);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+}
+
 // Rows wider than kMaxHeldColsBackward: dx (and dresidual) by one workgroup a row.
 template <typename T, typename TR, bool DROP>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
@@ -419,8 +448,12 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
         for (int64_t col = threadIdx.x * 8; col < cols; col += 8192) {
             const int valid = (int)(cols - col < 8 ? cols - col : 8);
             float v[8], g[8], w[8];
+            uint32_t kept = 0;
             load8(x + col, valid, v);
             load8(dy + col, valid, g);
+            if constexpr (DROP)
+                kept = keep8((uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng), a.threshold);
+            if constexpr (DROP && sizeof(TR) == 2) add_residual<TR>(a, row, col, valid, kept, v);
             if (a.w) load_param8<T>(a.w, a.wf32, (int)col, valid, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -433,15 +466,14 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) g[j] = rstd * (g[j] - m1 - v[j] * m2);
                 if constexpr (DROP) {
-                    if (a.res) {
+                    if (a.dz) {
                         float r[8];
-                        load8((const TR*)a.res + row * a.ldr + col, valid, r);
+                        load8((const TR*)a.dz + row * a.lddz + col, valid, r);
 #pragma unroll
                         for (int j = 0; j < 8; ++j) g[j] += r[j];
                     }
                     store8((TR*)a.z + row * a.ldz + col, valid, g);
-                    drop8(g, (uint64_t)row * (uint32_t)((cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng),
-                          a.threshold, a.scale);
+                    drop8(g, kept, a.scale);
                 }
                 store8((T*)a.y + row * a.ldy + col, valid, g);
             }
@@ -456,7 +488,7 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
 
 // Parameter gradients of rows wider than kMaxHeldColsBackward: 64 chunks of 8 columns by 4 waves;
 // the rows are dealt to gridDim.y workgroups and their waves in turn, one partial a workgroup.
-template <typename T, typename TR>
+template <typename T, typename TR, bool DROP>
 __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
     __shared__ float comb[3 * 64 * 16];
     const int t = threadIdx.x & 63, part = threadIdx.x >> 6;
@@ -471,6 +503,9 @@ __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
             float v[8], g[8];
             load8((const TR*)a.x + row * a.ldx + col, valid, v);
             load8((const T*)a.dy + row * a.lddy + col, valid, g);
+            if constexpr (DROP && sizeof(TR) == 2)
+                add_residual<TR>(a, row, col, valid,
+                                 keep8((uint64_t)row * (uint32_t)((a.cols - 1) / 8 + 1) + (uint64_t)(col / 8), drop_key(a.rng), a.threshold), v);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 s[0][j] += g[j] * ((v[j] - mean) * rstd);
@@ -571,7 +606,7 @@ hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
         OTF_NB(512, 512, 4);
     } else {
         norm_backward_long_kernel<T, TR, DROP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
-        if (WG) norm_param_long_kernel<T, TR><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
+        if (WG) norm_param_long_kernel<T, TR, DROP><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
     }
 #undef OTF_NB
     if (WG && (grid > 1 || !held)) {
@@ -735,7 +770,7 @@ static int norm_backward_call(NormArgs& a, bool drop, int32_t dtype, int32_t rdt
     }
     if (!a.x || !a.dy || !a.y || !a.mean || !a.rstd || a.ldx < cols || a.lddy < cols || a.ldy < cols) return OTF_EINVAL;
     if (!elem_aligned(a.x, rdtype) || !elem_aligned(a.dy, dtype) || !elem_aligned(a.y, dtype) ||
-        !elem_aligned(a.res, rdtype) || !elem_aligned(a.z, rdtype) || !elem_aligned(a.mean, OTF_F32) ||
+        !elem_aligned(a.z, rdtype) || !elem_aligned(a.mean, OTF_F32) ||
         !elem_aligned(a.rstd, OTF_F32))
         return OTF_EINVAL;
     const size_t need = (a.dw || a.db) ? otf_layer_norm_backward_workspace_size(rows, cols) : 0;
@@ -763,15 +798,22 @@ int otf_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t
 }
 
 int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void* dz, int64_t lddz, const void* z,
-                                        int64_t ldz, int32_t dtype, int32_t rdtype, const void* weight,
-                                        int32_t wdtype, const float* mean, const float* rstd, double p,
-                                        const int64_t* rng, int64_t rows, int64_t cols, void* dx, int64_t lddx,
-                                        void* dresidual, int64_t lddr, void* dweight, void* dbias, void* workspace,
+                                        int64_t ldz, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                        int32_t dtype, int32_t rdtype, const void* weight, int32_t wdtype,
+                                        const float* mean, const float* rstd, double p, const int64_t* rng,
+                                        int64_t rows, int64_t cols, void* dx, int64_t lddx, void* dresidual,
+                                        int64_t lddr, void* dweight, void* dbias, void* workspace,
                                         size_t workspace_bytes, otf_stream_t stream) {
     NormArgs a{};
     if (!drop_params(p, a.threshold, a.scale)) return OTF_EINVAL;
-    if (rows > 0 && (!rng || (uintptr_t)rng % 8 || !dresidual || lddr < cols || (dz && lddz < cols))) return OTF_EINVAL;
-    a.dy = dy, a.lddy = lddy, a.res = dz, a.ldr = lddz, a.x = z, a.ldx = ldz, a.w = weight;
+    const bool again = rdtype != OTF_F32;
+    if (rows > 0) {
+        if (!rng || (uintptr_t)rng % 8 || !dresidual || lddr < cols || (dz && lddz < cols)) return OTF_EINVAL;
+        if (again && (!residual || ldr < cols || !elem_aligned(residual, rdtype))) return OTF_EINVAL;
+        if (!elem_aligned(dz, rdtype)) return OTF_EINVAL;
+    }
+    a.dy = dy, a.lddy = lddy, a.dz = dz, a.lddz = lddz, a.w = weight;
+    a.x = again ? x : z, a.ldx = again ? ldx : ldz, a.res = residual, a.ldr = ldr;
     a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd), a.rng = rng;
     a.y = dx, a.ldy = lddx, a.z = dresidual, a.ldz = lddr, a.dw = dweight, a.db = dbias;
     return norm_backward_call(a, true, dtype, rdtype, wdtype, rows, cols, workspace, workspace_bytes, stream);

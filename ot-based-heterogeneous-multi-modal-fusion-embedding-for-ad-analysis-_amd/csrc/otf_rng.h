@@ -37,20 +37,23 @@ __device__ __forceinline__ void philox4x32_10(uint64_t index, const DropKey& key
     out[0] = c0, out[1] = c1, out[2] = c2, out[3] = c3;
 }
 
-// v of eight consecutive columns: v * scale where the column's 16-bit field reaches
-// `threshold`, else an exact 0 (a select: what is dropped may be inf or NaN).  16 bits an
-// element halve the generator's work against a 32-bit word each; the probability is the
-// multiple of 2^-16 nearest to the asked one, and `scale` is that multiple's, so the
-// expectation is exact.
-__device__ __forceinline__ void drop8(float (&v)[8], uint64_t index, const DropKey& key, uint32_t threshold,
-                                      float scale) {
-    uint32_t w[4];
+// Bit j: column j of eight is kept, its 16-bit field reaching `threshold`.  16 bits an element
+// halve the generator's work against a 32-bit word each; the probability is the multiple of 2^-16
+// nearest to the asked one, and the scale is that multiple's, so the expectation is exact.
+__device__ __forceinline__ uint32_t keep8(uint64_t index, const DropKey& key, uint32_t threshold) {
+    uint32_t w[4], m = 0;
     philox4x32_10(index, key, w);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const uint32_t field = (j & 1) ? w[j >> 1] >> 16 : w[j >> 1] & 0xffffu;
-        v[j] = field >= threshold ? v[j] * scale : 0.0f;
+        m |= field >= threshold ? 1u << j : 0u;
     }
+    return m;
+}
+// kept columns scaled, the others an exact 0 (a select: what is dropped may be inf or NaN)
+__device__ __forceinline__ void drop8(float (&v)[8], uint32_t kept, float scale) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (kept >> j) & 1 ? v[j] * scale : 0.0f;
 }
 
 // host: probability -> threshold (of 65536) and scale; p < 1 always keeps something

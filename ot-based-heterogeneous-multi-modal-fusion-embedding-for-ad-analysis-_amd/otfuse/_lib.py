@@ -184,7 +184,8 @@ _SIGS = {
                                                _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "otf_dropout_add_layer_norm": (ctypes.c_int, [_vp, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32, _dbl, _dbl, _vp,
                                                   _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
-    "otf_dropout_add_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _vp, _i32,
+    "otf_dropout_add_layer_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64,
+                                                           _i32, _i32, _vp, _i32,
                                                            _vp, _vp, _dbl, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
                                                            _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "otf_gated_ffn_saved_size": (ctypes.c_size_t, [_i64, _i64, _i32]),

@@ -263,11 +263,14 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, p, rng, eps, cols, wdt):
         ctx.set_materialize_grads(False)
-        y, z, stats = _add_norm_call(_rows(x.detach(), cols), _rows(residual.detach(), cols), _dense(weight),
-                                     _dense(bias), wdt, p, rng, eps, True)
+        x2, r2 = _rows(x.detach(), cols), _rows(residual.detach(), cols)
+        y, z, stats = _add_norm_call(x2, r2, _dense(weight), _dense(bias), wdt, p, rng, eps, True)
         z = z.view(x.shape)
-        ctx.save_for_backward(z, weight, stats, rng)
-        ctx.cols, ctx.wdt, ctx.p, ctx.dtype = cols, wdt, p, x.dtype
+        # a float32 z is the normalised sum itself; a rounded one is not: keep what it is the sum of
+        kept = (z,) if z.dtype == torch.float32 else (x if x2.data_ptr() == x.data_ptr() else x2,
+                                                       residual if r2.data_ptr() == residual.data_ptr() else r2)
+        ctx.save_for_backward(weight, stats, rng, *kept)
+        ctx.cols, ctx.wdt, ctx.p, ctx.dtype, ctx.rdtype = cols, wdt, p, x.dtype, z.dtype
         return y.view(x.shape), z
 
     @staticmethod
@@ -275,26 +278,29 @@ class _DropoutAddLayerNorm(torch.autograd.Function):
     def backward(ctx, dy, dz):
         if dy is None and dz is None:
             return (None,) * 9
-        z, weight, stats, rng = ctx.saved_tensors
+        weight, stats, rng, *kept = ctx.saved_tensors
         need, cols = ctx.needs_input_grad, ctx.cols
-        z2, w = _rows(z, cols), _dense(weight)
-        rows, dev = z2.shape[0], z2.device
+        shape, dev = (dz if dy is None else dy).shape, stats.device
+        kept, w = [_rows(t, cols) for t in kept], _dense(weight)
+        rows = stats.shape[1]
         if dy is None:
-            dy = torch.zeros(z.shape, dtype=ctx.dtype, device=dev)
+            dy = torch.zeros(shape, dtype=ctx.dtype, device=dev)
         dy2, dz2 = _rows(dy, cols), None if dz is None else _rows(dz, cols)
         dx = torch.empty((rows, cols), dtype=ctx.dtype, device=dev)
-        dr = torch.empty((rows, cols), dtype=z.dtype, device=dev)
+        dr = torch.empty((rows, cols), dtype=ctx.rdtype, device=dev)
         dw, db = _param_grads(cols, ctx.wdt, dev, need[2], need[3])
         ws, size = _norm_workspace(rows, cols, dev, need[2] or need[3])
+        z2, x2, r2 = (kept[0], None, None) if len(kept) == 1 else (None, *kept)
+        ld = lambda t: 0 if t is None else _ld(t)
         with _on(dev):
             L.check(L.lib().otf_dropout_add_layer_norm_backward(
-                dy2.data_ptr(), _ld(dy2), L.ptr(dz2), 0 if dz2 is None else _ld(dz2), z2.data_ptr(), _ld(z2),
-                _EMB_DT[ctx.dtype], _EMB_DT[z.dtype], L.ptr(w), _EMB_DT[ctx.wdt], stats.data_ptr(),
+                dy2.data_ptr(), _ld(dy2), L.ptr(dz2), ld(dz2), L.ptr(z2), ld(z2), L.ptr(x2), ld(x2), L.ptr(r2), ld(r2),
+                _EMB_DT[ctx.dtype], _EMB_DT[ctx.rdtype], L.ptr(w), _EMB_DT[ctx.wdt], stats.data_ptr(),
                 stats.data_ptr() + 4 * rows, ctx.p, rng.data_ptr(), rows, cols, dx.data_ptr(), cols, dr.data_ptr(),
                 cols, L.ptr(dw), L.ptr(db), L.ptr(ws), size, L.stream_handle(dev)),
                 "otf_dropout_add_layer_norm_backward")
-        return (dx.view(z.shape) if need[0] else None, dr.view(z.shape) if need[1] else None, dw, db, None, None,
-                None, None, None)
+        return (dx.view(shape) if need[0] else None, dr.view(shape) if need[1] else None, dw, db, None, None, None,
+                None, None)
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
@@ -303,7 +309,8 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torc
     """``z = residual + dropout(x)``, ``y = layer_norm(z)``; returns ``(y, z)``.
 
     residual and z: x's type or float32 (a 32-bit residual stream under 16-bit layers); y: x's
-    type, of z as it is stored.  ``rng`` may be None where ``p`` is 0."""
+    type, of the float32 sum.  ``rng`` may be None where ``p`` is 0.  Backward keeps a float32 z,
+    else x and residual."""
     _input(x, "x")
     _input(residual, "residual")
     _same_device(x, residual=residual)

@@ -256,7 +256,7 @@ def test_dropout_add_layer_norm(dev, dt, rt, rows, cols, p):
     xd, rd, wd, bd, dyd, dzd = (t.detach().double().cpu() for t in (x, res, w, b, dy, dz))
     s = xd * f + rd
     _within(z, s, half(T[rt]) * s.abs() + 4 * U * ((xd * f).abs() + rd.abs()))
-    zd = z.detach().double().cpu()   # y is the norm of z as stored
+    zd = s   # y is the norm of the float32 sum: within 2 u of s an element, which the row sums' bound holds
     yr, xhat, rstd = plain.layer_norm(zd, wd, bd, 1e-5)
     g, dw, db = plain.layer_norm_backward(dyd, xhat, rstd, wd)
     ty, tg, tw, tb = _norm_tolerance(zd, wd, dyd, half(T[dt]), 0, U, yr, xhat, rstd, g, dw, db)

@@ -107,10 +107,12 @@ def test_dropout_add_layer_norm_refuses(clib):
                dict(rdt=L.OTF_F16), dict(ldz=7), dict(ldr=7), dict(z=P + 2), dict(dt=L.OTF_F64)):
         assert fwd(**kw) == L.OTF_EINVAL, kw
     assert fwd(rows=0, x=None) == L.OTF_OK
-    def bwd(dy=P, z=P, p=0.1, rng=P, dx=P, dr=P, dz=P, lddz=8):
-        return lib.otf_dropout_add_layer_norm_backward(dy, 8, dz, lddz, z, 8, L.OTF_BF16, L.OTF_F32, P, L.OTF_F32, P, P, p,
-                                                       rng, 2, 8, dx, 8, dr, 8, None, None, None, 0, None)
-    for kw in (dict(dy=None), dict(z=None), dict(p=-1.0), dict(rng=None), dict(dx=None), dict(dr=None), dict(lddz=7)):
+    def bwd(dy=P, z=P, x=None, r=None, ldr=8, rdt=L.OTF_F32, p=0.1, rng=P, dx=P, dr=P, dz=P, lddz=8):
+        return lib.otf_dropout_add_layer_norm_backward(dy, 8, dz, lddz, z, 8, x, 8, r, ldr, L.OTF_BF16, rdt, P, L.OTF_F32, P,
+                                                       P, p, rng, 2, 8, dx, 8, dr, 8, None, None, None, 0, None)
+    for kw in (dict(dy=None), dict(z=None), dict(p=-1.0), dict(rng=None), dict(dx=None), dict(dr=None), dict(lddz=7),
+               dict(dz=P + 2), dict(rdt=L.OTF_BF16), dict(rdt=L.OTF_BF16, x=P), dict(rdt=L.OTF_BF16, r=P),
+               dict(rdt=L.OTF_BF16, x=P, r=P, ldr=7), dict(rdt=L.OTF_BF16, x=P, r=P + 1)):
         assert bwd(**kw) == L.OTF_EINVAL, kw
 
 
