@@ -845,25 +845,43 @@ struct Product {
 
 constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 
-// Tile 256 x 256 (16-bit operands) where that fills the chip, else 128 x 128, else 64 x 64; K
-// split into slabs where even the small tiles leave most of it idle.
+// Tile side and slabs of K, by the least estimated time.  A CU holds one tile of 256, two of 128 or
+// three of 64; a K-tile then takes it c microseconds (less where it holds fewer), a tile's start and
+// results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted to bf16 products of 64 to
+// 4096 rows by 512 to 4096 and 1408 to 11264 columns, each run with all three sides:
+//   gate and up 1024 x 2048 x 5632   62 / 91 / 85 us with 256 / 128 / 64   (176, 704, 2816 tiles)
+//               64 x 4096 x 11264    85 / 93 / 58                          (88, 176, 352)
+//   dh          1024 x 2048 x 5632   78 / 50 / 60                          (88, 352, 1408)
+//   dx          1024 x 2048 x 5632   87 / 65 / 101, the first two with 16 and 4 slabs
+//   dWg and dWu 777 x 1024 x 2752    36 / 20 / 28
 struct Plan {
-    int tm, tn, splits;
+    int side, splits;
 };
 Plan plan_product(const Product& p, int elem) {
     const GemmArgs& a = p.a;
-    auto tiles = [&](int t) {
-        const int64_t m = (a.M + t - 1) / t, n = p.epi == kGatedForward ? (2 * (int64_t)a.N + t - 1) / t : (a.N + t - 1) / t;
-        return m * n * a.batch;
-    };
-    const bool whole = (p.tra || a.a.k % 64 == 0) && (p.trb || a.b.k % 64 == 0);
-    const int side = elem == 2 && whole && tiles(256) >= kCus ? 256 : tiles(128) >= kCus ? 128 : 64;
-    int splits = 1;
-    if (p.epi == kStore) {
-        const int64_t ktiles = (int64_t)(a.a.k + kTileBytes / elem - 1) / (kTileBytes / elem) * a.segments, t = tiles(side);
-        while (t * splits * 2 <= 2 * kCus && ktiles / (splits * 2) >= 4) splits *= 2;
+    const bool whole = elem == 2 && (p.tra || a.a.k % 64 == 0) && (p.trb || a.b.k % 64 == 0);
+    const int depth = kTileBytes / elem;
+    const int64_t ktiles = (int64_t)((a.a.k + depth - 1) / depth) * a.segments;
+    Plan best{64, 1};
+    double least = 1e30;
+    for (int side : {256, 128, 64}) {
+        if (side == 256 && !whole) continue;
+        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : 3;
+        const double c = elem == 2 ? (side == 256 ? 1.35 : side == 128 ? 1.1 : 0.75) : (side == 128 ? 4.2 : 1.9);
+        const double e = side == 256 ? 14.0 : side == 128 ? 11.0 : 5.0;
+        const int64_t rows = (a.M + side - 1) / side, width = p.epi == kGatedForward ? side / 2 : side;
+        const int64_t tiles = rows * ((a.N + width - 1) / width) * a.batch, slots = (int64_t)kCus * per_cu;
+        for (int splits = 1; splits <= 32; splits *= 2) {
+            if (splits > 1 && (p.epi != kStore || tiles * splits > slots || ktiles / splits < 4)) break;
+            const double full = (double)(tiles * splits) / slots;
+            const double rounds = full < 1.0 ? 1.0 : side == 64 ? full : (double)((tiles + slots - 1) / slots);
+            const double speed = per_cu == 1 ? 1.0 : 0.5 + 0.5 * (full < 1.0 ? full : 1.0);
+            double us = rounds * ((double)((ktiles + splits - 1) / splits) * c * speed + e);
+            if (splits > 1) us += 4.0 + (double)splits * a.batch * a.M * a.N * 4.0 * (1 / 6.4e6 + 1 / 4.0e6);
+            if (us < least) least = us, best = Plan{side, splits};
+        }
     }
-    return Plan{side, side, splits};
+    return best;
 }
 size_t slab_bytes(const Product& p, const Plan& q) {
     return q.splits > 1 ? (size_t)q.splits * p.a.batch * p.a.M * (size_t)up8(p.a.N) * 4 : 0;
@@ -872,13 +890,13 @@ size_t slab_bytes(const Product& p, const Plan& q) {
 template <typename T, bool TRA, bool TRB, int EPI>
 hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     a.splits = q.splits;
-    a.tiles_m = (a.M + q.tm - 1) / q.tm;
-    const int cols = EPI == kGatedForward ? q.tn / 2 : q.tn;
+    a.tiles_m = (a.M + q.side - 1) / q.side;
+    const int cols = EPI == kGatedForward ? q.side / 2 : q.side;
     a.tiles_n = (a.N + cols - 1) / cols;
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
-    if (q.tm == 256) {
+    if (q.side == 256) {
         if constexpr (sizeof(T) == 2) ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
-    } else if (q.tm == 128)
+    } else if (q.side == 128)
         ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
     else
         ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
@@ -973,7 +991,12 @@ GemmArgs product_args(const Operand& a, const Operand& b, int64_t M, int64_t N, 
     return g;
 }
 
-constexpr int kFewRows = 16;   // one MFMA tile of rows
+// The few-rows kernel takes one MFMA tile of rows.  With more of them its reads of x grow beside
+// the weights': bf16, d = 4096, f = 11264, 16 rows 71 us against 57 for the tiles, 1 row 53; d = 1024,
+// f = 4096, 16 rows 16.0 against 18.6.  float32 tiles are slower everywhere up to 16 rows.
+bool few_rows(int64_t rows, int64_t d, int64_t f, int es) {
+    return rows <= 16 && (es == 4 || rows * d * f <= (int64_t)1 << 26);
+}
 
 int check_ffn(const otf_ffn_args* o) {
     if (!o) return OTF_EINVAL;
@@ -1007,7 +1030,7 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
         sv = carve_saved(o->saved, b.n, b.f64, b.es);
     else
         sv.h = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
-    if (b.n <= kFewRows) {
+    if (few_rows(b.n, b.d, b.f, b.es)) {
         *need = b.ws.used;
         if (!run) return OTF_OK;
         const unsigned g1 = (unsigned)(b.f64 / 16), g2 = (unsigned)((b.d + 15) / 16);
