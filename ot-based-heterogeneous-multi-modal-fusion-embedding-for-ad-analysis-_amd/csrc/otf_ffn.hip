@@ -125,7 +125,8 @@ template <typename T, int R> __device__ __forceinline__ int swz_t(int k) {
 }
 
 template <typename T, bool TR, int R, int NT> struct Tile {
-    static constexpr int BYTES = R * kTileBytes, CHUNKS = BYTES / 16, PER = (CHUNKS + NT - 1) / NT;
+    static constexpr int BYTES = R * kTileBytes, CHUNKS = BYTES / 16, PER = CHUNKS / NT;
+    static_assert(CHUNKS % NT == 0, "every wave issues the same loads");
     static constexpr int BK = kTileBytes / (int)sizeof(T);
     static constexpr int CPR = R * (int)sizeof(T) / 16;   // layout T: chunks of a k row
     uint32_t off[PER];
@@ -146,43 +147,18 @@ template <typename T, bool TR, int R, int NT> struct Tile {
             }
         }
     }
-    // K-tile kt of the operand whose first row (K) / column (T) is at `base`, of which `mn`
-    // remain, into LDS at `dst`
-    __device__ __forceinline__ void stage(const char* base, int64_t ld, int mn, int kvalid, int kt, char* dst) const {
+    // A K-tile into LDS at `dst`: `bytes` from `base` on are readable and a lane past them gets
+    // zeros.  MASK: so does one past the first `left` bytes of K (layout K, whose rows are followed
+    // by the next ones).
+    template <bool MASK> __device__ __forceinline__ void put(const char* base, uint32_t bytes, int left, char* dst) const {
 #ifdef __HIP_DEVICE_COMPILE__   // the buffer builtins: the host pass drops the launch stubs of kernels that reach them
-        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        if constexpr (TR) {
-            const int rows = min(kvalid - kt * BK, BK);
-            const int64_t bytes = rows > 0 && mn > 0 ? (rows - 1) * ld + (int64_t)min(mn, R) * (int)sizeof(T) : 0;
-            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)kt * BK * ld), 0, (int)bytes, kRsrcFlags);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if ((i + 1) * NT <= CHUNKS || i * NT + wave * 64 < CHUNKS)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                        r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16, off[i], 0, 0, 0);
-        } else {
-            const int left = kvalid * (int)sizeof(T) - kt * kTileBytes;   // bytes of K still ahead
-            const int64_t bytes = mn > 0 && left > 0 ? (int64_t)(min(mn, R) - 1) * ld + left : 0;
-            const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)kt * kTileBytes), 0, (int)bytes, kRsrcFlags);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if ((i + 1) * NT <= CHUNKS || i * NT + wave * 64 < CHUNKS)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                        r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16,
-                        kb[i] < left ? off[i] : 0xfffffff0u, 0, 0, 0);
-        }
-#endif
-    }
-    // the same with the range worked out by the caller: `bytes` from `base` on are readable, a lane
-    // past them gets zeros.  Whole K-tiles only in layout K.
-    __device__ __forceinline__ void put(const char* base, uint32_t bytes, char* dst) const {
-#ifdef __HIP_DEVICE_COMPILE__
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, kRsrcFlags);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16, off[i], 0, 0, 0);
+                r, (__attribute__((address_space(3))) void*)(dst + (i * NT + wave * 64) * 16), 16,
+                MASK && kb[i] >= left ? 0xfffffff0u : off[i], 0, 0, 0);
 #endif
     }
     // fragment of the 16 rows from r0, K half s
@@ -259,7 +235,7 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
         if (n < a.N) *reinterpret_cast<f32x4*>(c + n) = acc0;
         if (n2 < a.N) *reinterpret_cast<f32x4*>(c + n2) = acc1;
     } else if constexpr (EPI == kGatedForward) {
-        if (n >= a.N) return;   // N, ldh multiples of 64
+        if (n >= a.N) return;   // N, ldh whole K-tiles
         const int64_t o = (int64_t)m * a.ldh + n;
         f32x4 h;
 #pragma unroll
@@ -303,14 +279,42 @@ __device__ __forceinline__ void tile_of(int id, int count, int tiles_m, int tile
     tn = in / rows;
 }
 
-// A kernel argument that a loop selects by a run-time index: in registers, so that the loop does
-// not load it again
-__device__ __forceinline__ const char* held(const char* p) {
-#ifdef __HIP_DEVICE_COMPILE__
-    asm volatile("" : "+s"(p));
-#endif
-    return p;
-}
+// A tile's place in its operand, moved on by a K-tile with each load, so that a load costs a few
+// scalar instructions.  Readable bytes: layout K, the valid rows whole (the K-tile may start anywhere
+// in them; a row past them starts past that range); layout T, the K-tile's rows, fewer in a
+// segment's last one.  Past the end of K nothing is readable: a load brings zeros.
+template <typename T, bool TR, int R> struct Cursor {
+    static constexpr int BK = kTileBytes / (int)sizeof(T);
+    const char *p, *second;
+    int64_t step;
+    uint32_t bytes, bytes_last;
+    int nk, total, kbytes, left;
+    // K-tiles from k0 on of `segments` runs of nk: the first from p0, the second from p1
+    __device__ __forceinline__ void init(const Operand& o, const char* p0, const char* p1, int mn, int nk_, int total_, int k0) {
+        nk = nk_, total = total_;
+        const int64_t rows = min(mn, R);
+        step = TR ? BK * o.ld : kTileBytes;
+        const int last = o.k - (nk - 1) * BK;
+        if (TR) {
+            bytes = mn > 0 ? (uint32_t)((BK - 1) * o.ld + rows * (int)sizeof(T)) : 0u;
+            bytes_last = mn > 0 && last > 0 ? (uint32_t)((last - 1) * o.ld + rows * (int)sizeof(T)) : 0u;
+        } else {
+            bytes = bytes_last = mn > 0 ? (uint32_t)((rows - 1) * o.ld + (int64_t)o.k * (int)sizeof(T)) : 0u;
+        }
+        const int skip = k0 >= nk ? k0 - nk : k0;
+        p = (k0 >= nk ? p1 : p0) + skip * step;
+        second = p1;
+        kbytes = o.k * (int)sizeof(T);
+        left = kbytes - skip * kTileBytes;
+    }
+    template <bool MASK, typename TILE> __device__ __forceinline__ void load(const TILE& tile, int kt, char* dst) {
+        uint32_t n = kt >= total ? 0u : bytes;
+        if (TR && (kt == nk - 1 || kt == total - 1)) n = bytes_last;
+        tile.template put<MASK && !TR>(p, n, left, dst);
+        p = kt == nk - 1 ? second : p + step;
+        if (MASK && !TR) left = kt == nk - 1 ? kbytes : left - kTileBytes;
+    }
+};
 
 // N fragments of layout T over a whole K-tile: f[block][half of K][four k], from this lane's
 // addresses of the blocks' first k, rows of ROW bytes (the permutation of a row's chunks is the
@@ -394,7 +398,6 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
     using TB = Tile<T, TRB, TH, NT>;
     constexpr int BUF = TA::BYTES + 2 * TB::BYTES;
     constexpr int LOADS = TA::PER + 2 * TB::PER;   // a wave's, a K-tile
-    static_assert(TA::CHUNKS % NT == 0 && TB::CHUNKS % NT == 0, "every wave issues the same loads");
     __shared__ __attribute__((aligned(16))) char smem[S * BUF];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / WGN, wn = wid % WGN;
 
@@ -413,16 +416,23 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 
     const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
     const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
-    const char *pa0 = held(a.a.p[a.batch > 1 ? z : 0] + am), *pa1 = held(a.a.p[1] + am);   // a batch has one segment
-    const char *pb0 = held(a.b.p[0] + bn), *pb1 = held(a.b.p[1] + bn);
+    const char *a0 = a.a.p[a.batch > 1 ? z : 0] + am, *a1 = a.a.p[1] + am;   // a batch has one segment
+    const char *b0 = a.b.p[0] + bn, *b1 = a.b.p[1] + bn;
+    Cursor<T, TRA, TM> ca;
+    ca.init(a.a, a0, a1, a.a.mn - m0, nk, total, k0);
+    Cursor<T, TRB, TH> cb[2];
+    if constexpr (EPI == kGatedForward) {
+        cb[0].init(a.b, b0, b0, a.b.mn - n0, nk, total, k0);
+        cb[1].init(a.b, b1, b1, a.b.mn - n0, nk, total, k0);
+    } else {
+        cb[0].init(a.b, b0, b1, a.b.mn - n0, nk, total, k0);
+        cb[1].init(a.b, b0 + bh, b1 + bh, a.b.mn - n0 - TH, nk, total, k0);
+    }
     auto stage = [&](int kt, int buf) {
-        const int seg = a.segments > 1 && kt >= nk ? 1 : 0, k = kt - seg * nk;
         char* dst = smem + buf * BUF;
-        ta.stage(seg ? pa1 : pa0, a.a.ld, a.a.mn - m0, a.a.k, k, dst);
-        const char* b0 = EPI != kGatedForward && seg ? pb1 : pb0;
-        const char* b1 = EPI == kGatedForward ? pb1 : b0 + bh;
-        tb.stage(b0, a.b.ld, a.b.mn - n0, a.b.k, k, dst + TA::BYTES);
-        tb.stage(b1, a.b.ld, EPI == kGatedForward ? a.b.mn - n0 : a.b.mn - n0 - TH, a.b.k, k, dst + TA::BYTES + TB::BYTES);
+        ca.template load<true>(ta, kt, dst);
+        cb[0].template load<true>(tb, kt, dst + TA::BYTES);
+        cb[1].template load<true>(tb, kt, dst + TA::BYTES + TB::BYTES);
     };
 
     f32x4 acc[2][RB][RA];
@@ -532,51 +542,23 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     tb.init(a.b.ld);
     const int nk = (a.a.k + TA::BK - 1) / TA::BK, total = nk * a.segments;
     const int k0 = (int)((int64_t)total * split / a.splits), k1 = (int)((int64_t)total * (split + 1) / a.splits);
-    // A half-tile's place in its operand, moved on by a K-tile with each load.  Readable bytes:
-    // layout K, the valid rows whole (the K-tile may start anywhere in them, and a row past them
-    // starts past that range); layout T, the K-tile's rows, less in a segment's last one.
-    struct Cursor {
-        const char *p, *second;
-        int64_t step;
-        uint32_t bytes, bytes_last;
-    };
-    auto cursor = [&](const Operand& o, bool tr, const char* p0, const char* p1, int mn, int kvalid) {
-        Cursor c;
-        const int64_t rows = min(mn, 128);
-        c.step = tr ? TA::BK * o.ld : kTileBytes;
-        const int last = kvalid - (nk - 1) * TA::BK;   // layout T: its own k (a padded A may be deeper)
-        if (tr) {
-            c.bytes = mn > 0 ? (uint32_t)((TA::BK - 1) * o.ld + rows * 2) : 0u;
-            c.bytes_last = mn > 0 && last > 0 ? (uint32_t)((last - 1) * o.ld + rows * 2) : 0u;
-        } else {
-            c.bytes = c.bytes_last = mn > 0 ? (uint32_t)((rows - 1) * o.ld + (int64_t)kvalid * 2) : 0u;
-        }
-        const int skip = k0 >= nk ? k0 - nk : k0;
-        c.p = (k0 >= nk ? p1 : p0) + skip * c.step;
-        c.second = p1;
-        return c;
-    };
     const int za = a.batch > 1 ? z : 0;   // a batch has one segment
     const int64_t am = TRA ? (int64_t)m0 * 2 : (int64_t)m0 * a.a.ld, ah = TRA ? 256 : 128 * a.a.ld;
     const int64_t bn = TRB ? (int64_t)n0 * 2 : (int64_t)n0 * a.b.ld, bh = TRB ? 256 : 128 * a.b.ld;
     const char *a0 = a.a.p[za] + am, *a1 = a.a.p[1] + am, *b0 = a.b.p[0] + bn, *b1 = a.b.p[1] + bn;
-    Cursor ca[2] = {cursor(a.a, TRA, a0, a1, a.a.mn - m0, a.a.k), cursor(a.a, TRA, a0 + ah, a1 + ah, a.a.mn - m0 - 128, a.a.k)};
-    Cursor cb[2];
+    Cursor<T, TRA, 128> ca[2];
+    ca[0].init(a.a, a0, a1, a.a.mn - m0, nk, total, k0);
+    ca[1].init(a.a, a0 + ah, a1 + ah, a.a.mn - m0 - 128, nk, total, k0);
+    Cursor<T, TRB, 128> cb[2];
     if constexpr (EPI == kGatedForward) {
-        cb[0] = cursor(a.b, TRB, b0, b0, a.b.mn - n0, a.b.k);
-        cb[1] = cursor(a.b, TRB, b1, b1, a.b.mn - n0, a.b.k);
+        cb[0].init(a.b, b0, b0, a.b.mn - n0, nk, total, k0);
+        cb[1].init(a.b, b1, b1, a.b.mn - n0, nk, total, k0);
     } else {
-        cb[0] = cursor(a.b, TRB, b0, b1, a.b.mn - n0, a.b.k);
-        cb[1] = cursor(a.b, TRB, b0 + bh, b1 + bh, a.b.mn - n0 - 128, a.b.k);
+        cb[0].init(a.b, b0, b1, a.b.mn - n0, nk, total, k0);
+        cb[1].init(a.b, b0 + bh, b1 + bh, a.b.mn - n0 - 128, nk, total, k0);
     }
-    auto advance = [&](const auto& tile, Cursor& c, bool tr, int kt, char* dst) {
-        uint32_t bytes = kt >= total ? 0u : c.bytes;
-        if (tr && (kt == nk - 1 || kt == total - 1)) bytes = c.bytes_last;
-        tile.put(c.p, bytes, dst);
-        c.p = kt == nk - 1 ? c.second : c.p + c.step;
-    };
-    auto stage_a = [&](int h, int kt, int buf) { advance(ta, ca[h], TRA, kt, smem + buf * BUF + h * HT); };
-    auto stage_b = [&](int h, int kt, int buf) { advance(tb, cb[h], TRB, kt, smem + buf * BUF + (2 + h) * HT); };
+    auto stage_a = [&](int h, int kt, int buf) { ca[h].template load<false>(ta, kt, smem + buf * BUF + h * HT); };
+    auto stage_b = [&](int h, int kt, int buf) { cb[h].template load<false>(tb, kt, smem + buf * BUF + (2 + h) * HT); };
 
     uint32_t xa[4], xb[2];   // layout T: addresses in the first buffer
 #pragma unroll
@@ -771,7 +753,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
     }
     if (!live) return;
     const int n = n0 + kc * 4;
-    if constexpr (GATED) {   // ldo a multiple of 64, columns up to it written (zeros past N)
+    if constexpr (GATED) {   // ldo whole K-tiles, columns up to it written (zeros past N)
         f32x4 h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -822,7 +804,7 @@ template <typename T> __global__ __launch_bounds__(256) void ffn_zero_kernel(T* 
 
 // ------------------------------------------------------------------------------------- host
 int64_t up8(int64_t x) { return (x + 7) / 8 * 8; }
-int64_t up64(int64_t x) { return (x + 63) / 64 * 64; }   // a whole 16-bit K-tile
+int64_t up_ktile(int64_t x, int es) { return (x + kTileBytes / es - 1) / (kTileBytes / es) * (kTileBytes / es); }
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 size_t esize(int32_t t) { return t == OTF_F32 ? 4 : 2; }
 
@@ -889,6 +871,9 @@ size_t slab_bytes(const Product& p, const Plan& q) {
 
 template <typename T, bool TRA, bool TRB, int EPI>
 hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
+    // both operands run over the same K-tiles: the cursors shorten only the last one's rows
+    constexpr int depth = kTileBytes / (int)sizeof(T);
+    if ((a.a.k + depth - 1) / depth != (a.b.k + depth - 1) / depth) return hipErrorInvalidValue;
     a.splits = q.splits;
     a.tiles_m = (a.M + q.side - 1) / q.side;
     const int cols = EPI == kGatedForward ? q.side / 2 : q.side;
@@ -896,9 +881,17 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
     if (q.side == 256) {
         if constexpr (sizeof(T) == 2) ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
-    } else if (q.side == 128)
+    } else if (q.side == 128) {
+        // a third buffer where a CU has only one tile: 4096 x 1024 x 4096, down product, 82 -> 56 us.  With
+        // a T operand it gains nothing, and two tiles of two buffers are faster where there are more.
+        if constexpr (!TRA && !TRB) {
+            if ((int64_t)grid.x * grid.y <= kCus) {
+                ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
+                return hipGetLastError();
+            }
+        }
         ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
-    else
+    } else
         ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
     return hipGetLastError();
 }
@@ -922,14 +915,14 @@ hipError_t run_store(const Product& p, float* slab, hipStream_t s) {
 struct Block {
     const otf_ffn_args* o;
     int es;
-    int64_t n, d, f, f64;   // f64: leading dimension of the hidden buffers, zeros past f
+    int64_t n, d, f, fk;    // fk: f in whole K-tiles, the hidden buffers' leading dimension, zeros past f
     bool whole;             // operands copied to whole K-tiles (large products of ragged widths)
     Operand x{}, wg{}, wu{}, wd{}, dy{};   // k: columns there are, zeros past the caller's
     PackArgs pack{};
     Carver ws{};
 
     Block(const otf_ffn_args* args, int elem, void* workspace) : o(args), es(elem) {
-        n = o->rows, d = o->d, f = o->f, f64 = up64(f);
+        n = o->rows, d = o->d, f = o->f, fk = up_ktile(f, es);
         // ragged widths: a copy costs two passes over the operands, and pays where the products are large
         whole = es == 2 && ((n + 255) / 256) * ((f + 127) / 128) >= kCus;
         ws.base = (char*)workspace;
@@ -943,7 +936,7 @@ struct Block {
         v.ld = ld * es;
         v.k = (int)cols;
         if (copy) {
-            const int64_t ldd = up64(cols);
+            const int64_t ldd = up_ktile(cols, es);
             void* dst = ws.take((size_t)(rows * ldd * es));
             pack.item[pack.count++] = PackItem{p, dst, ld, ldd, rows, cols, pack.total};
             pack.total += rows * (ldd / 8);
@@ -1015,30 +1008,30 @@ struct Saved {
     float *g, *u;
     char* h;
 };
-Saved carve_saved(void* p, int64_t n, int64_t f64, int es) {
+Saved carve_saved(void* p, int64_t n, int64_t fk, int es) {
     char* b = (char*)p;
-    const size_t wide = up256((size_t)(n * f64) * 4);
+    const size_t wide = up256((size_t)(n * fk) * 4);
     return Saved{(float*)b, (float*)(b + wide), b + 2 * wide};
 }
-size_t saved_bytes(int64_t n, int64_t f64, int es) { return 2 * up256((size_t)(n * f64) * 4) + up256((size_t)(n * f64 * es)); }
+size_t saved_bytes(int64_t n, int64_t fk, int es) { return 2 * up256((size_t)(n * fk) * 4) + up256((size_t)(n * fk * es)); }
 
 // forward: the workspace it needs in *need; runs where run is set
 template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
     Saved sv{};
     if (o->saved)
-        sv = carve_saved(o->saved, b.n, b.f64, b.es);
+        sv = carve_saved(o->saved, b.n, b.fk, b.es);
     else
-        sv.h = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
+        sv.h = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
     if (few_rows(b.n, b.d, b.f, b.es)) {
         *need = b.ws.used;
         if (!run) return OTF_OK;
-        const unsigned g1 = (unsigned)(b.f64 / 16), g2 = (unsigned)((b.d + 15) / 16);
+        const unsigned g1 = (unsigned)((b.fk + 15) / 16), g2 = (unsigned)((b.d + 15) / 16);
         ffn_few_kernel<T, true, 4><<<g1, 256, 0, s>>>((const T*)o->x, o->ldx, (int)b.n, (const T*)o->w_gate,
                                                        (const T*)o->w_up, o->ldw_in, (int)b.d, (int)b.f, o->activation,
-                                                       (T*)sv.h, b.f64, sv.g, sv.u);
+                                                       (T*)sv.h, b.fk, sv.g, sv.u);
         OTF_HIP(hipGetLastError());
-        ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.f64, (int)b.n, (const T*)o->w_down, nullptr,
+        ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.fk, (int)b.n, (const T*)o->w_down, nullptr,
                                                         o->ldw_down, (int)b.f, (int)b.d, 0, (T*)o->y, o->ldy, nullptr,
                                                         nullptr);
         return check_hip(hipGetLastError());
@@ -1047,10 +1040,10 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     b.weights_in();
     b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
     const int kin = b.x.k < b.wg.k ? b.x.k : b.wg.k;   // what is copied ends in zeros
-    Product in{false, false, kGatedForward, product_args(by_rows(b.x, b.n, kin), by_rows(b.wg, b.f, kin), b.n, b.f64, nullptr, 0)};
+    Product in{false, false, kGatedForward, product_args(by_rows(b.x, b.n, kin), by_rows(b.wg, b.f, kin), b.n, b.fk, nullptr, 0)};
     in.a.b.p[1] = b.wu.p[0];
-    in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.f64;
-    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.f64, b.es, b.n, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
+    in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.fk;
+    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.fk, b.es, b.n, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
     float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es)));
     *need = b.ws.used;
     if (!run) return OTF_OK;
@@ -1062,25 +1055,25 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
 
 template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
-    const Saved sv = carve_saved(o->saved, b.n, b.f64, b.es);
+    const Saved sv = carve_saved(o->saved, b.n, b.fk, b.es);
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
-    char* dg = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
-    char* du = (char*)b.ws.take((size_t)(b.n * b.f64 * b.es));
+    char* dg = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
+    char* du = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
     b.operand(b.dy, o->dy, o->lddy, b.n, b.d);
     if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
     if (wx) b.weights_in();
     if (win) b.operand(b.x, o->x, o->ldx, b.n, b.d);
     // dh = dy Wd: K = d, the rows of Wd
-    Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.f64, nullptr, 0)};
-    mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.f64;
+    Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.fk, nullptr, 0)};
+    mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.fk;
     // dx = dg Wg + du Wu: two segments of K = f, the rows of the weights
-    Product px{false, true, kStore, product_args(buffer_operand(dg, b.f64, b.es, b.n, b.f64), by_columns(b.wg, b.f), b.n, b.d, o->dx, o->lddx)};
+    Product px{false, true, kStore, product_args(buffer_operand(dg, b.fk, b.es, b.n, b.fk), by_columns(b.wg, b.f), b.n, b.d, o->dx, o->lddx)};
     px.a.a.p[1] = du, px.a.b.p[1] = b.wu.p[0], px.a.segments = 2;
     // dWg, dWu = dg^T x, du^T x: a batch of two, K = rows
-    Product pi{true, true, kStore, product_args(buffer_operand(dg, b.f64, b.es, b.f64, b.n), by_columns(b.x, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
+    Product pi{true, true, kStore, product_args(buffer_operand(dg, b.fk, b.es, b.fk, b.n), by_columns(b.x, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
     pi.a.a.p[1] = du, pi.a.c[1] = o->dw_up, pi.a.batch = 2;
     // dWd = dy^T h
-    Product pd{true, true, kStore, product_args(by_columns(b.dy, b.n), buffer_operand(sv.h, b.f64, b.es, b.f64, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
+    Product pd{true, true, kStore, product_args(by_columns(b.dy, b.n), buffer_operand(sv.h, b.fk, b.es, b.fk, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
     size_t slab = 0;   // one after another on the stream: they share it
     auto more = [&](const Product& p) { const size_t k = slab_bytes(p, plan_product(p, b.es)); slab = k > slab ? k : slab; };
     if (wx) more(px);
@@ -1122,7 +1115,7 @@ extern "C" {
 
 size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype) {
     if (rows <= 0 || f <= 0) return 0;
-    return saved_bytes(rows, up64(f), (int)esize(dtype));
+    return saved_bytes(rows, up_ktile(f, (int)esize(dtype)), (int)esize(dtype));
 }
 
 size_t otf_gated_ffn_workspace_size(const otf_ffn_args* o) {

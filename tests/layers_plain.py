@@ -18,14 +18,14 @@ def threshold(p):
     return 65536 if p >= 1 else min(65535, int(math.floor(p * 65536 + 0.5)))
 
 
-def factor(rows, cols, p, seed, offset):
-    """keep / (1 - p) as float64 (rows, cols), on the CPU"""
+def factor(rows, cols, p, seed, offset, first=0):
+    """keep / (1 - p) of rows first... as float64 (rows, cols), on the CPU"""
     t = threshold(p)
     scale = 0.0 if t == 65536 else 65536.0 / (65536 - t)
     groups = (cols + 7) // 8
     off, key = (offset & 0xFFFFFFFF, (offset >> 32) & 0xFFFFFFFF), (seed & 0xFFFFFFFF, (seed >> 32) & 0xFFFFFFFF)
     # word arithmetic on int64 tensors: 32 x 32 -> 64 products by 16-bit halves
-    at = torch.arange(rows * groups, dtype=torch.int64)
+    at = torch.arange(first * groups, (first + rows) * groups, dtype=torch.int64)
     m32 = 0xFFFFFFFF
 
     def mul(a, m):

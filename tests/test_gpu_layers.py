@@ -411,6 +411,63 @@ def test_gated_feed_forward_against_differences(dev):
             assert abs(diff - want) <= 5e-3 * scale, (act, i, diff, want)
 
 
+# ------------------------------------------------------------------ past 2^31 elements
+def test_rowwise_layers_past_32_bit_offsets(dev):
+    """2.2e9 elements: the first and the last rows against the plain forms."""
+    from otfuse import layers
+    rows, cols, p, seed, offset = 270001, 8200, 0.25, 99, 3
+    rng = layers.rng_state(seed, offset, dev)
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=dev)
+    block = _randn(dev, 1, 1009, cols, dtype=torch.bfloat16)
+    for i in range(0, rows, 1009):
+        x[i:i + 1009] = block[:min(1009, rows - i)]
+    y, z = layers.dropout_add_layer_norm(x, x, p=p, rng=rng)
+    d = layers.dropout(x, p, rng)
+    n = layers.layer_norm(x)
+    one, zero, h = torch.ones(cols, dtype=torch.float64), torch.zeros(cols, dtype=torch.float64), half(torch.bfloat16)
+    for first in (0, rows - 5):
+        f = plain.factor(5, cols, p, seed, offset, first)
+        xs = x[first:first + 5].double().cpu()
+        _within(d[first:first + 5], xs * f, (h + 3 * U) * (xs * f).abs())
+        s = xs * f + xs
+        _within(z[first:first + 5], s, h * s.abs() + 4 * U * 2 * xs.abs() * (1 + f))
+        for got, v in ((y, s), (n, xs)):
+            want, xhat, rstd = plain.layer_norm(v, one, zero, 1e-5)
+            e = xhat.abs() + rstd * v.abs().mean(1, keepdim=True)
+            _within(got[first:first + 5], want, h * want.abs() + 128 * U * e)
+    del y, z, d
+    leaf = x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(layers.layer_norm(leaf), leaf, n)
+    for first in (0, rows - 5):
+        v = x.detach()[first:first + 5].double().cpu()
+        dy = n[first:first + 5].double().cpu()
+        _, xhat, rstd = plain.layer_norm(v, one, zero, 1e-5)
+        want, _, _ = plain.layer_norm_backward(dy, xhat, rstd, one)
+        tol = _norm_tolerance(v, one, dy, 0, h, 0, xhat, xhat, rstd, want, zero, zero)[1]
+        _within(dx[first:first + 5], want, tol)
+
+
+def test_gated_feed_forward_past_32_bit_offsets(dev):
+    """2.3e9 hidden values: y and dx of the last rows, which no other row reaches."""
+    from otfuse import layers
+    rows, d, f, t = 220001, 128, 10304, torch.bfloat16
+    w = [_randn(dev, i, *s, dtype=t, scale=k) for i, s, k in ((2, (f, d), 0.09), (3, (f, d), 0.09), (4, (d, f), 0.01))]
+    x = torch.zeros(rows, d, dtype=t, device=dev)
+    x[-70:] = _randn(dev, 1, 70, d, dtype=t)
+    dy = torch.zeros(rows, d, dtype=t, device=dev)
+    dy[-70:] = _randn(dev, 5, 70, d, dtype=t)
+    args = [v.requires_grad_(True) for v in (x, *w)]
+    y = layers.gated_feed_forward(*args)
+    grads = torch.autograd.grad(y, args, dy)
+    ref = plain.gated_feed_forward(x.detach()[-70:].double(), *(v.detach().double() for v in w), "silu", dy[-70:].double())
+    depth = 2 * (d + f) + 70 + 16
+    _close(y[-70:], ref[0], 3, t, depth)
+    _close(grads[0][-70:], ref[1], 7, t, depth)
+    assert torch.count_nonzero(y[:-70]) == 0 and torch.count_nonzero(grads[0][:-70]) == 0
+    for got, want, n in zip(grads[1:], ref[2:], (7, 7, 3)):   # only the last rows contribute
+        _close(got, want, n, t, depth)
+
+
 # ----------------------------------------------------------------- streams, graphs, the block
 def _step(leaves, rng, dy):
     from otfuse import layers
