@@ -680,6 +680,7 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const float* __restrict__
     const int64_t zm = i / per, n = (i - zm * per) * 4, z = zm / M, m = zm - z * M;
     if (n >= N) return;
     f32x4 s = *reinterpret_cast<const f32x4*>(slab + zm * ldp + n);
+#pragma unroll 8   // the additions are in order, the loads need not wait for each other
     for (int k = 1; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(slab + ((int64_t)k * batch * M + zm) * ldp + n);
     T* c = (z ? c1 : c0) + m * ldc;
     const bool vec = (ldc & 3) == 0 && ((uintptr_t)(z ? c1 : c0) & (4 * sizeof(T) - 1)) == 0;
@@ -827,8 +828,8 @@ struct Product {
 
 constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 
-// Tile side and slabs of K, by the least estimated time.  A CU holds one tile of 256, two of 128 or
-// three of 64; a K-tile then takes it c microseconds (less where it holds fewer), a tile's start and
+// Tile side and slabs of K, by the least estimated time.  A CU holds one tile of 256, two of 128,
+// three of 64 or five of 16 by 64; a K-tile then takes it c microseconds (less where it holds fewer), a tile's start and
 // results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted to bf16 products of 64 to
 // 4096 rows by 512 to 4096 and 1408 to 11264 columns, each run with all three sides:
 //   gate and up 1024 x 2048 x 5632   62 / 91 / 85 us with 256 / 128 / 64   (176, 704, 2816 tiles)
@@ -846,17 +847,18 @@ Plan plan_product(const Product& p, int elem) {
     const int64_t ktiles = (int64_t)((a.a.k + depth - 1) / depth) * a.segments;
     Plan best{64, 1};
     double least = 1e30;
-    for (int side : {256, 128, 64}) {
-        if (side == 256 && !whole) continue;
-        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : 3;
-        const double c = elem == 2 ? (side == 256 ? 1.35 : side == 128 ? 1.1 : 0.75) : (side == 128 ? 4.2 : 1.9);
+    for (int side : {256, 128, 64, 16}) {   // 16: 16 rows by 64 columns
+        if ((side == 256 && !whole) || (side == 16 && (p.tra || a.M > 16))) continue;
+        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : side == 64 ? 3 : 5;
+        const double c = elem == 2 ? (side == 256 ? 1.35 : side == 128 ? 1.1 : side == 64 ? 0.75 : 0.6) : (side == 128 ? 4.2 : side == 64 ? 1.9 : 0.8);
         const double e = side == 256 ? 14.0 : side == 128 ? 11.0 : 5.0;
-        const int64_t rows = (a.M + side - 1) / side, width = p.epi == kGatedForward ? side / 2 : side;
+        const int64_t across = side == 16 ? 64 : side, width = p.epi == kGatedForward ? across / 2 : across;
+        const int64_t rows = (a.M + side - 1) / side;
         const int64_t tiles = rows * ((a.N + width - 1) / width) * a.batch, slots = (int64_t)kCus * per_cu;
         for (int splits = 1; splits <= 32; splits *= 2) {
             if (splits > 1 && (p.epi != kStore || tiles * splits > slots || ktiles / splits < 4)) break;
             const double full = (double)(tiles * splits) / slots;
-            const double rounds = full < 1.0 ? 1.0 : side == 64 ? full : (double)((tiles + slots - 1) / slots);
+            const double rounds = full < 1.0 ? 1.0 : side <= 64 ? full : (double)((tiles + slots - 1) / slots);
             const double speed = per_cu == 1 ? 1.0 : 0.5 + 0.5 * (full < 1.0 ? full : 1.0);
             double us = rounds * ((double)((ktiles + splits - 1) / splits) * c * speed + e);
             if (splits > 1) us += 4.0 + (double)splits * a.batch * a.M * a.N * 4.0 * (1 / 6.4e6 + 1 / 4.0e6);
@@ -876,7 +878,7 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     if ((a.a.k + depth - 1) / depth != (a.b.k + depth - 1) / depth) return hipErrorInvalidValue;
     a.splits = q.splits;
     a.tiles_m = (a.M + q.side - 1) / q.side;
-    const int cols = EPI == kGatedForward ? q.side / 2 : q.side;
+    const int across = q.side == 16 ? 64 : q.side, cols = EPI == kGatedForward ? across / 2 : across;
     a.tiles_n = (a.N + cols - 1) / cols;
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
     if (q.side == 256) {
@@ -891,8 +893,11 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
             }
         }
         ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
-    } else
+    } else if (q.side == 16) {   // up to 16 rows: a taller tile's MFMAs would be spent on rows that are not there
+        if constexpr (!TRA) ffn_gemm_kernel<T, TRA, TRB, 16, 64, 1, 2, 3, EPI><<<grid, 128, 0, s>>>(a);
+    } else {
         ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
+    }
     return hipGetLastError();
 }
 

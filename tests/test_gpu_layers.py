@@ -287,7 +287,7 @@ def _close(got, want, roundings, dtype, depth):
     assert excess <= 0, f"an element is {excess:.3e} beyond eight deviations"
 
 
-FFNS = [(1, 8, 16), (1, 1, 1), (1, 1000, 333), (3, 64, 96), (16, 130, 100), (16, 512, 1032), (17, 72, 136), (33, 250, 71),
+FFNS = [(9, 640, 48), (16, 48, 2100), (12, 1100, 600), (1, 8, 16), (1, 1, 1), (1, 1000, 333), (3, 64, 96), (16, 130, 100), (16, 512, 1032), (17, 72, 136), (33, 250, 71),
         (64, 64, 64), (130, 512, 264), (200, 1000, 334), (257, 136, 1100), (5, 2048, 40), (700, 40, 2056), (513, 1024, 1408)]
 
 
@@ -409,6 +409,18 @@ def test_gated_feed_forward_against_differences(dev):
             diff, want = (loss(step) - loss(-step)) / (2 * step), float(g.double().square().sum())
             scale = max(want, float(g.norm()) * float(dy.norm()) * float(layers.gated_feed_forward(*args, activation=act).norm()) / float(args[i].norm()))
             assert abs(diff - want) <= 5e-3 * scale, (act, i, diff, want)
+
+
+def test_second_derivatives_are_refused(dev):
+    from otfuse import layers
+    x = torch.randn(4, 16, device=dev, requires_grad=True)
+    w = torch.randn(24, 16, device=dev, requires_grad=True)
+    rng = layers.rng_state(1, 2, dev)
+    for y in (layers.dropout(x, 0.1, rng), layers.layer_norm(x), layers.dropout_add_layer_norm(x, x, p=0.1, rng=rng)[0],
+              layers.gated_feed_forward(x, w, w, w.t())):
+        (g,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
 
 
 # ------------------------------------------------------------------ past 2^31 elements

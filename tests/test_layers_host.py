@@ -159,3 +159,12 @@ def test_python_entry_points_refuse_host_tensors():
                  lambda: layers.gated_feed_forward(x, torch.zeros(4, 8), torch.zeros(4, 8), torch.zeros(8, 4))):
         with pytest.raises(TypeError, match="device tensor"):
             call()
+
+
+def test_missing_nodes_fail_loudly(monkeypatch, tmp_path):
+    from otfuse import _lib as L
+    from otfuse import layers
+    monkeypatch.setattr(layers, "NODES_PATH", str(tmp_path / "missing.so"))
+    monkeypatch.setattr(layers, "_nodes", None)
+    with pytest.raises(L.OtfError):
+        layers._native()
