@@ -316,61 +316,20 @@ template <typename T, bool TR, int R> struct Cursor {
     }
 };
 
+// A transposed LDS read.  The pointer is restrict-qualified: with no alias information on the read
+// the compiler waits for every LDS-writing load in flight before it; the order that matters here is
+// kept by this file's own waits and barriers.
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+__device__ __forceinline__ s16x4 read_tr4(lds_s16x4* __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
 // N fragments of layout T over a whole K-tile: f[block][half of K][four k], from this lane's
 // addresses of the blocks' first k, rows of ROW bytes (the permutation of a row's chunks is the
-// same four rows on and half a K-tile on).  In assembly because the compiler waits for every load
-// in flight before such a read; the wait for the reads is part of the block, so nothing after it
-// can use a register whose read is under way.
-template <int N, int ROW, int OFF> __device__ __forceinline__ void read_tr(const uint32_t (&p)[N], s16x4 (&f)[N][2][2]) {
-    static_assert(N == 1 || N == 2 || N == 4, "blocks");
-#ifdef __HIP_DEVICE_COMPILE__
-    if constexpr (N == 1)
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %4 offset:%5\n\t"
-            "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-            "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
-            "ds_read_b64_tr_b16 %3, %4 offset:%8\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1])
-            : "v"(p[0]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
-            : "memory");
-    if constexpr (N == 2)
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %8 offset:%10\n\t"
-            "ds_read_b64_tr_b16 %1, %8 offset:%11\n\t"
-            "ds_read_b64_tr_b16 %2, %8 offset:%12\n\t"
-            "ds_read_b64_tr_b16 %3, %8 offset:%13\n\t"
-            "ds_read_b64_tr_b16 %4, %9 offset:%10\n\t"
-            "ds_read_b64_tr_b16 %5, %9 offset:%11\n\t"
-            "ds_read_b64_tr_b16 %6, %9 offset:%12\n\t"
-            "ds_read_b64_tr_b16 %7, %9 offset:%13\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]), "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1])
-            : "v"(p[0]), "v"(p[1]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
-            : "memory");
-    if constexpr (N == 4)
-        asm volatile(
-            "ds_read_b64_tr_b16 %0, %16 offset:%20\n\t"
-            "ds_read_b64_tr_b16 %1, %16 offset:%21\n\t"
-            "ds_read_b64_tr_b16 %2, %16 offset:%22\n\t"
-            "ds_read_b64_tr_b16 %3, %16 offset:%23\n\t"
-            "ds_read_b64_tr_b16 %4, %17 offset:%20\n\t"
-            "ds_read_b64_tr_b16 %5, %17 offset:%21\n\t"
-            "ds_read_b64_tr_b16 %6, %17 offset:%22\n\t"
-            "ds_read_b64_tr_b16 %7, %17 offset:%23\n\t"
-            "ds_read_b64_tr_b16 %8, %18 offset:%20\n\t"
-            "ds_read_b64_tr_b16 %9, %18 offset:%21\n\t"
-            "ds_read_b64_tr_b16 %10, %18 offset:%22\n\t"
-            "ds_read_b64_tr_b16 %11, %18 offset:%23\n\t"
-            "ds_read_b64_tr_b16 %12, %19 offset:%20\n\t"
-            "ds_read_b64_tr_b16 %13, %19 offset:%21\n\t"
-            "ds_read_b64_tr_b16 %14, %19 offset:%22\n\t"
-            "ds_read_b64_tr_b16 %15, %19 offset:%23\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(f[0][0][0]), "=&v"(f[0][0][1]), "=&v"(f[0][1][0]), "=&v"(f[0][1][1]), "=&v"(f[1][0][0]), "=&v"(f[1][0][1]), "=&v"(f[1][1][0]), "=&v"(f[1][1][1]), "=&v"(f[2][0][0]), "=&v"(f[2][0][1]), "=&v"(f[2][1][0]), "=&v"(f[2][1][1]), "=&v"(f[3][0][0]), "=&v"(f[3][0][1]), "=&v"(f[3][1][0]), "=&v"(f[3][1][1])
-            : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "n"(OFF), "n"(OFF + 4 * ROW), "n"(OFF + 32 * ROW), "n"(OFF + 36 * ROW)
-            : "memory");
-#endif
+// same four rows on and half a K-tile on)
+template <int N, int ROW> __device__ __forceinline__ void read_tr(const uint32_t (&p)[N], uint32_t offset, s16x4 (&f)[N][2][2]) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            f[t][q >> 1][q & 1] = read_tr4((lds_s16x4*)(uintptr_t)(p[t] + offset + (q >> 1) * 32 * ROW + (q & 1) * 4 * ROW));
 }
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -462,36 +421,27 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
         const char* sb = sa + TA::BYTES;
         Frags<T, RA> fa;
         Frags<T, RB> fb[2];
-        if constexpr ((TRA || TRB) && sizeof(T) == 2) stage(kt + S - 1, next);
         if constexpr (TRA && sizeof(T) == 2) {
-            uint32_t p[RA];
-#pragma unroll
-            for (int i = 0; i < RA; ++i) p[i] = xa[i] + buf * BUF;
-            read_tr<RA, TM * 2, 0>(p, fa.h);
+            read_tr<RA, TM * 2>(xa, buf * BUF, fa.h);
         } else {
 #pragma unroll
             for (int i = 0; i < RA; ++i)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) fa.f[i][s] = TA::frag(sa, (wm * RA + i) * 16, s, lane);
         }
-        if constexpr (TRB && sizeof(T) == 2) {
-            uint32_t p[RB];
 #pragma unroll
-            for (int j = 0; j < RB; ++j) p[j] = xb[j] + buf * BUF;
-            read_tr<RB, TH * 2, 0>(p, fb[0].h);
-            read_tr<RB, TH * 2, TB::BYTES>(p, fb[1].h);
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (TRB && sizeof(T) == 2) {
+                read_tr<RB, TH * 2>(xb, buf * BUF + h * TB::BYTES, fb[h].h);
+            } else {
 #pragma unroll
                 for (int j = 0; j < RB; ++j)
 #pragma unroll
                     for (int s = 0; s < 2; ++s) fb[h].f[j][s] = TB::frag(sb + h * TB::BYTES, (wn * RB + j) * 16, s, lane);
+            }
         }
-        if constexpr (!((TRA || TRB) && sizeof(T) == 2)) {
-            asm volatile("" ::: "memory");
-            stage(kt + S - 1, next);
-        }
+        asm volatile("" ::: "memory");
+        stage(kt + S - 1, next);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -570,8 +520,7 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     auto read_a = [&](int buf, auto half) {
         constexpr int H = decltype(half)::value;
         if constexpr (TRA) {
-            const uint32_t p[4] = {xa[0] + buf * BUF, xa[1] + buf * BUF, xa[2] + buf * BUF, xa[3] + buf * BUF};
-            read_tr<4, 256, H * HT>(p, fa.h);
+            read_tr<4, 256>(xa, buf * BUF + H * HT, fa.h);
         } else {
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -582,8 +531,7 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
     auto read_b = [&](int buf, auto half) {
         constexpr int H = decltype(half)::value;
         if constexpr (TRB) {
-            const uint32_t p[2] = {xb[0] + buf * BUF, xb[1] + buf * BUF};
-            read_tr<2, 256, (2 + H) * HT>(p, fb[H].h);
+            read_tr<2, 256>(xb, buf * BUF + (2 + H) * HT, fb[H].h);
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -620,24 +568,20 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
         constexpr int P = decltype(parity)::value;
         using First = std::integral_constant<int, P>;
         using Second = std::integral_constant<int, 1 - P>;
-        if constexpr (TRA) stage_a(1, kt + 1, 1 - P);
         read_a(P, I0{});
-        if constexpr (!TRA) stage_a(1, kt + 1, 1 - P);
+        stage_a(1, kt + 1, 1 - P);
         wait_loads<10>();
         quadrant(I0{}, First{});
-        if constexpr (TRB) stage_b(P, kt + 2, P);
         read_b(P, Second{});
-        if constexpr (!TRB) stage_b(P, kt + 2, P);
+        stage_b(P, kt + 2, P);
         wait_loads<10>();
         quadrant(I0{}, Second{});
-        if constexpr (TRA) stage_a(0, kt + 2, P);
         read_a(P, I1{});
-        if constexpr (!TRA) stage_a(0, kt + 2, P);
+        stage_a(0, kt + 2, P);
         wait_loads<10>();
         quadrant(I1{}, Second{});
-        if constexpr (TRB) stage_b(1 - P, kt + 2, P);
-        read_b(1 - P, Second{});
-        if constexpr (!TRB) stage_b(1 - P, kt + 2, P);
+        read_b(1 - P, Second{});   // the next K-tile's first half, into the registers this one is done with
+        stage_b(1 - P, kt + 2, P);
         wait_loads<10>();
         quadrant(I1{}, First{});
     };
