@@ -613,7 +613,8 @@ int otf_emd_solve(int32_t nprob, const otf_emd_problem* probs, int64_t max_pivot
  * rng: DEVICE pointer to two int64, {seed, offset}.  The mask of an element depends on
  *   (seed, offset, row, column, cols) alone (Philox4x32-10, 16 bits an element), so backward
  *   makes the forward's mask again from the same two words; calls that must not share a mask
- *   take different seeds or offsets.  A captured graph reads the words at every replay.
+ *   take different seeds or offsets.  A captured graph reads the words at every replay.  May be
+ *   NULL where p rounds to 0: nothing is generated then.
  * p: 0 <= p <= 1, rounded to a multiple t of 2^-16 (p < 1 keeps t <= 65535); kept elements are
  *   scaled by 65536 / (65536 - t), dropped ones are an exact 0 whatever they held.
  * weight, bias: cols elements of wdtype (the input's type or OTF_F32), each may be NULL.
@@ -662,7 +663,8 @@ int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void
  * saved: what backward needs of the forward call (the gate and up products and h), opaque,
  *   otf_gated_ffn_saved_size bytes, 16-byte aligned; NULL in inference.  workspace: 16-byte
  *   aligned, at least ..._workspace_size bytes of the SAME arguments (pointers included: an
- *   operand whose rows are not 16-byte aligned is copied to one whose are); it may be reused
+ *   operand whose rows are not 16-byte aligned is copied to one whose are; d * f, rows * d and
+ *   rows * f at most 2^34); it may be reused
  *   as soon as the call's work on the stream is done.
  * Backward reads dy, x, the weights and saved.  dx NULL: not computed; dw_gate and dw_up go
  *   together (one leading dimension), dw_down by itself.

@@ -743,8 +743,8 @@ template <typename T> __global__ __launch_bounds__(256) void ffn_pack_kernel(Pac
     store8((T*)it.dst + row * it.ldd + col, 8, v);
 }
 template <typename T> __global__ __launch_bounds__(256) void ffn_zero_kernel(T* p, int64_t rows, int64_t cols, int64_t ld) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i < rows * cols) p[i / cols * ld + i % cols] = (T)0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * cols; i += (int64_t)gridDim.x * 256)
+        p[i / cols * ld + i % cols] = (T)0.0f;
 }
 
 // ------------------------------------------------------------------------------------- host
@@ -947,6 +947,9 @@ int check_ffn(const otf_ffn_args* o) {
     if (o->rows < 0 || o->d <= 0 || o->f <= 0) return OTF_EINVAL;
     // 32-bit element counts of a row tile and of the K extents
     if (o->rows > INT32_MAX / 8 || o->d > (1 << 20) || o->f > (1 << 20)) return OTF_EUNSUPPORTED;
+    // and 32-bit thread counts of the launches
+    const int64_t wide = o->d > o->f ? o->d : o->f, most = (int64_t)1 << 34;
+    if (o->d * o->f > most || o->rows * wide > most) return OTF_EUNSUPPORTED;
     return OTF_OK;
 }
 // leading dimensions: 256 rows within a 31-bit byte offset
@@ -1040,7 +1043,8 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
 }
 
 template <typename T> hipError_t zero_rows(void* p, int64_t rows, int64_t cols, int64_t ld, hipStream_t s) {
-    ffn_zero_kernel<T><<<(unsigned)((rows * cols + 255) / 256), 256, 0, s>>>((T*)p, rows, cols, ld);
+    const int64_t n = (rows * cols + 255) / 256;
+    ffn_zero_kernel<T><<<(unsigned)(n < 65536 ? n : 65536), 256, 0, s>>>((T*)p, rows, cols, ld);
     return hipGetLastError();
 }
 

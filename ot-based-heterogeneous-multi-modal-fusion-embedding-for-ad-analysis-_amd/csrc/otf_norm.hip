@@ -67,13 +67,29 @@ __device__ __forceinline__ void load_param8(const void* p, int wf32, int col, in
         load8((const T*)p + col, valid, v);
 }
 
-// Sum of NV values over the TPR threads of a row.  TPR = 64: one wave, no LDS.  Else one
+// x over lanes whose ids differ below bit TPR (a row's lanes), or from it on (the rows of a wave)
+template <int TPR> __device__ __forceinline__ float row_lanes_sum(float x) {
+    if constexpr (TPR > 1) x += wave_xor<float, 1>(x);
+    if constexpr (TPR > 2) x += wave_xor<float, 2>(x);
+    if constexpr (TPR > 4) x += wave_xor<float, 4>(x);
+    if constexpr (TPR > 8) x += wave_xor<float, 8>(x);
+    if constexpr (TPR > 16) x += wave_xor<float, 16>(x);
+    if constexpr (TPR > 32) x += wave_xor<float, 32>(x);
+    return x;
+}
+
+// A launch's workgroups, more than 2^20 of them in rows of 2^20: HIP counts a dimension's threads in
+// 32 bits.
+__device__ __forceinline__ int64_t block_id() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+dim3 blocks(int64_t n) { return n <= 1 << 20 ? dim3((unsigned)n) : dim3(1u << 20, (unsigned)((n + (1 << 20) - 1) >> 20)); }
+
+// Sum of NV values over the TPR threads of a row.  Up to 64: within a wave, no LDS.  Else one
 // barrier: `red` holds two generations of [wave][NV], and a wave can be at most one
 // reduction ahead of another.
 template <int TPR, int NV>
 __device__ __forceinline__ void row_sums(float (&s)[NV], float* red, int& gen) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s[i] = wave_sum(s[i]);
+    for (int i = 0; i < NV; ++i) s[i] = TPR >= 64 ? wave_sum(s[i]) : row_lanes_sum<TPR>(s[i]);
     if constexpr (TPR > 64) {
         constexpr int NW = TPR / 64;
         float* slot = red + gen * NW * NV;
@@ -102,7 +118,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, i
                                                       int64_t ldy, uint64_t total, uint32_t groups, int cols,
                                                       const int64_t* __restrict__ rng, uint32_t threshold,
                                                       float scale) {
-    const uint64_t g = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint64_t g = (uint64_t)block_id() * 256 + threadIdx.x;
     if (g >= total) return;
     int64_t ox, orr, oy;
     int valid = 8;
@@ -133,11 +149,11 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, i
 template <typename T, typename TR, bool DROP, int TPR, int CH>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_forward_kernel(NormArgs a) {
     constexpr int NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
-    __shared__ float red[2 * (TPR / 64)];
+    __shared__ float red[TPR > 64 ? 2 * (TPR / 64) : 1];
     int gen = 0;
     const int t = threadIdx.x % TPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (row >= a.rows) return;   // whole waves: RPB > 1 only where a wave is a row
+    const int64_t row = block_id() * RPB + threadIdx.x / TPR;
+    if (row >= a.rows) return;   // all of a row's threads; RPB > 1 only where they share a wave
     const int cols = a.cols;
     const T* x = (const T*)a.x + row * a.ldx;
     float v[CH][8];
@@ -209,7 +225,8 @@ template <typename T, typename TR, bool DROP>
 __global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormArgs a) {
     __shared__ float red[2 * 16];
     int gen = 0;
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_id();
+    if (row >= a.rows) return;
     const int cols = a.cols;
     const T* x = (const T*)a.x + row * a.ldx;
     TR* z = DROP ? (TR*)a.z + row * a.ldz : nullptr;
@@ -297,7 +314,7 @@ template <typename T, typename TR, bool DROP, bool WG, int NT, int TPR, int CH>
 __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
     constexpr int RPB = NT / TPR;
     __shared__ float red[TPR > 64 ? 4 * (TPR / 64) : 1];
-    __shared__ float comb[WG && RPB > 1 ? (RPB - 1) * 64 * 8 : 1];
+    __shared__ float comb[WG && RPB > 1 ? (NT / 64 - 1) * 64 * 8 : 1];
     int gen = 0;
     const int t = threadIdx.x % TPR, part = threadIdx.x / TPR;
     const int cols = a.cols;
@@ -400,20 +417,28 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
                 store_param_grad<T>(a, 0, col, gw[c]);
                 store_param_grad<T>(a, 1, col, gb[c]);
             }
-        } else {   // the workgroup's waves joined through LDS, a chunk of one gradient at a time
+        } else {   // a wave's rows joined by exchanges, the waves through LDS, a chunk of one gradient at a time
+            constexpr int NW = NT / 64;
+            const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
 #pragma unroll
             for (int i = 0; i < 2 * CH; ++i) {
                 float(&s)[8] = (i & 1) ? gb[i >> 1] : gw[i >> 1];
-                __syncthreads();
-                if (part > 0)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) comb[((part - 1) * 8 + j) * 64 + t] = s[j];
+                for (int j = 0; j < 8; ++j) {
+                    if constexpr (TPR <= 8) s[j] += wave_xor<float, 8>(s[j]);
+                    if constexpr (TPR <= 16) s[j] += wave_xor<float, 16>(s[j]);
+                    if constexpr (TPR <= 32) s[j] += wave_xor<float, 32>(s[j]);
+                }
+                __syncthreads();
+                if (wid > 0)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) comb[((wid - 1) * 8 + j) * 64 + lane] = s[j];
                 __syncthreads();
                 const int col = ((i >> 1) * TPR + t) * 8;
-                if (part == 0 && col < cols) {
-                    for (int p = 0; p < RPB - 1; ++p)
+                if (wid == 0 && lane < TPR && col < cols) {
+                    for (int p = 0; p < NW - 1; ++p)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) s[j] += comb[(p * 8 + j) * 64 + t];
+                        for (int j = 0; j < 8; ++j) s[j] += comb[(p * 8 + j) * 64 + lane];
                     store_param_grad<T>(a, i & 1, col, s);
                 }
             }
@@ -437,7 +462,8 @@ template <typename T, typename TR, bool DROP>
 __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
     __shared__ float red[2 * 16 * 2];
     int gen = 0;
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_id();
+    if (row >= a.rows) return;
     const int cols = a.cols;
     const TR* x = (const TR*)a.x + row * a.ldx;
     const T* dy = (const T*)a.dy + row * a.lddy;
@@ -554,9 +580,16 @@ template <typename T, typename TR, bool DROP>
 hipError_t norm_forward(const NormArgs& a, hipStream_t s) {
 #define OTF_NF(TPR, CH) norm_forward_kernel<T, TR, DROP, TPR, CH><<<grid, TPR > 256 ? TPR : 256, 0, s>>>(a)
     const int c = a.cols;
-    const bool wave = c <= 2048;
-    const unsigned grid = (unsigned)(wave ? (a.rows + 3) / 4 : a.rows);
-    if (c <= 512)
+    // narrow rows share a wave: with 64 lanes a row of 64 columns, 7 of 8 lanes would idle
+    const int per = c <= 64 ? 32 : c <= 128 ? 16 : c <= 256 ? 8 : c <= 2048 ? 4 : 1;
+    const dim3 grid = blocks((a.rows + per - 1) / per);
+    if (c <= 64)
+        OTF_NF(8, 1);
+    else if (c <= 128)
+        OTF_NF(16, 1);
+    else if (c <= 256)
+        OTF_NF(32, 1);
+    else if (c <= 512)
         OTF_NF(64, 1);
     else if (c <= 1024)
         OTF_NF(64, 2);
@@ -581,7 +614,7 @@ hipError_t norm_forward(const NormArgs& a, hipStream_t s) {
 // -> 25 us), until the partials' traffic counts (16384 x 2048 float32: 88 us, 82 with 512).
 int norm_backward_groups(int64_t rows, int64_t cols) {
     const bool held = cols <= kMaxHeldColsBackward;
-    const int64_t per = !held ? 64 : cols <= 1024 ? 4 : 1;
+    const int64_t per = !held ? 64 : cols <= 64 ? 32 : cols <= 128 ? 16 : cols <= 256 ? 8 : cols <= 1024 ? 4 : 1;
     const int64_t most = !held ? 32 : cols > 8192 ? 256 : cols > 1024 && cols <= 2048 && rows < 8192 ? 1024 : 512;
     const int64_t want = (rows + per - 1) / per;
     return (int)(want < most ? want : most);
@@ -592,7 +625,13 @@ hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
     const int c = a.cols, grid = norm_backward_groups(a.rows, c);
     const bool held = c <= kMaxHeldColsBackward;
 #define OTF_NB(NT, TPR, CH) norm_backward_kernel<T, TR, DROP, WG, NT, TPR, CH><<<grid, NT, 0, s>>>(a)
-    if (c <= 512) {
+    if (c <= 64) {
+        OTF_NB(256, 8, 1);
+    } else if (c <= 128) {
+        OTF_NB(256, 16, 1);
+    } else if (c <= 256) {
+        OTF_NB(256, 32, 1);
+    } else if (c <= 512) {
         OTF_NB(256, 64, 1);
     } else if (c <= 1024) {
         OTF_NB(256, 64, 2);
@@ -605,7 +644,7 @@ hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
     } else if (held) {
         OTF_NB(512, 512, 4);
     } else {
-        norm_backward_long_kernel<T, TR, DROP><<<(unsigned)a.rows, 1024, 0, s>>>(a);
+        norm_backward_long_kernel<T, TR, DROP><<<blocks(a.rows), 1024, 0, s>>>(a);
         if (WG) norm_param_long_kernel<T, TR, DROP><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
     }
 #undef OTF_NB
@@ -631,7 +670,7 @@ hipError_t dropout_launch(const void* x, int64_t ldx, const void* res, int64_t l
     const uint32_t groups = (uint32_t)((cols + 7) / 8);
     const uint64_t total = (uint64_t)rows * groups;
     const bool flat = cols % 8 == 0 && ldx == cols && ldy == cols && (!res || ldr == cols);
-    const unsigned grid = (unsigned)((total + 255) / 256);
+    const dim3 grid = blocks((int64_t)((total + 255) / 256));
 #define OTF_DK(RES, FLAT)                                                                                     \
     dropout_kernel<T, RES, FLAT><<<grid, 256, 0, s>>>((const T*)x, ldx, (const T*)res, ldr, (T*)y, ldy, total, \
                                                       groups, (int)cols, rng, threshold, scale)
@@ -688,11 +727,11 @@ int otf_dropout(const void* x, int64_t ldx, const void* residual, int64_t ldr, v
     float scale;
     if (rows < 0 || cols < 0 || !type16_or_32(dtype) || !drop_params(p, threshold, scale)) return OTF_EINVAL;
     if (rows == 0 || cols == 0) return OTF_OK;
-    if (!x || !y || !rng || ldx < cols || ldy < cols || (residual && ldr < cols)) return OTF_EINVAL;
+    if (!x || !y || (threshold && !rng) || ldx < cols || ldy < cols || (residual && ldr < cols)) return OTF_EINVAL;
     if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || !elem_aligned(residual, dtype)) return OTF_EINVAL;
     if ((uintptr_t)rng % 8) return OTF_EINVAL;
     if (cols > INT32_MAX - 8 || rows > INT64_MAX / ((cols + 7) / 8)) return OTF_EUNSUPPORTED;
-    if (rows * ((cols + 7) / 8) > (int64_t)256 * INT32_MAX) return OTF_EUNSUPPORTED;
+    if (rows * ((cols + 7) / 8) > (int64_t)1 << 42) return OTF_EUNSUPPORTED;   // of 8 elements each
     return by_type<false>(dtype, dtype, [&](auto* t, auto*) {
         using T = std::remove_pointer_t<decltype(t)>;
         return dropout_launch<T>(x, ldx, residual, ldr, y, ldy, rows, cols, threshold, scale, rng, (hipStream_t)stream);
@@ -729,7 +768,8 @@ int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const 
     if (!(eps >= 0.0) || (mean == nullptr) != (rstd == nullptr) || !drop_params(p, a.threshold, a.scale))
         return OTF_EINVAL;
     if (rows == 0) return OTF_OK;
-    if (!x || !residual || !y || !z || !rng || ldx < cols || ldr < cols || ldy < cols || ldz < cols) return OTF_EINVAL;
+    if (!x || !residual || !y || !z || (a.threshold && !rng)) return OTF_EINVAL;
+    if (ldx < cols || ldr < cols || ldy < cols || ldz < cols) return OTF_EINVAL;
     if (!elem_aligned(x, dtype) || !elem_aligned(y, dtype) || !elem_aligned(residual, rdtype) ||
         !elem_aligned(z, rdtype) || !elem_aligned(weight, wdtype) || !elem_aligned(bias, wdtype) ||
         !elem_aligned(mean, OTF_F32) || !elem_aligned(rstd, OTF_F32) || (uintptr_t)rng % 8)
@@ -808,7 +848,7 @@ int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void
     if (!drop_params(p, a.threshold, a.scale)) return OTF_EINVAL;
     const bool again = rdtype != OTF_F32;
     if (rows > 0) {
-        if (!rng || (uintptr_t)rng % 8 || !dresidual || lddr < cols || (dz && lddz < cols)) return OTF_EINVAL;
+        if ((a.threshold && !rng) || (uintptr_t)rng % 8 || !dresidual || lddr < cols || (dz && lddz < cols)) return OTF_EINVAL;
         if (again && (!residual || ldr < cols || !elem_aligned(residual, rdtype))) return OTF_EINVAL;
         if (!elem_aligned(dz, rdtype)) return OTF_EINVAL;
     }

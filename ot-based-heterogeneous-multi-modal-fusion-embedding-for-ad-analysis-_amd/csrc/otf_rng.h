@@ -15,8 +15,9 @@ struct DropKey {
     uint32_t k0, k1, o0, o1;
 };
 
-// rng: two int64, seed and offset (wave-uniform loads)
+// rng: two int64, seed and offset (wave-uniform loads); null where nothing is dropped
 __device__ __forceinline__ DropKey drop_key(const int64_t* rng) {
+    if (!rng) return DropKey{};
     const uint64_t seed = (uint64_t)rng[0], off = (uint64_t)rng[1];
     return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
 }
@@ -40,7 +41,9 @@ __device__ __forceinline__ void philox4x32_10(uint64_t index, const DropKey& key
 // Bit j: column j of eight is kept, its 16-bit field reaching `threshold`.  16 bits an element
 // halve the generator's work against a 32-bit word each; the probability is the multiple of 2^-16
 // nearest to the asked one, and the scale is that multiple's, so the expectation is exact.
+// A threshold of 0 (uniform) keeps all without the generator.
 __device__ __forceinline__ uint32_t keep8(uint64_t index, const DropKey& key, uint32_t threshold) {
+    if (threshold == 0) return 0xffu;
     uint32_t w[4], m = 0;
     philox4x32_10(index, key, w);
 #pragma unroll

@@ -51,6 +51,7 @@ int64_t ld(const Tensor& t) { return t.defined() ? std::max(t.stride(0), t.size(
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 Tensor dense(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }
+const int64_t* words(const Tensor& rng) { return rng.defined() ? rng.const_data_ptr<int64_t>() : nullptr; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && wants(*t); }
 
@@ -72,7 +73,7 @@ Tensor dropout_call(const Tensor& x, const Tensor& residual, double p, const Ten
     const Tensor x2 = rows_of(x, cols), r2 = residual.defined() ? rows_of(residual, cols) : Tensor();
     Tensor y = at::empty(x.sizes(), x.options());
     check(otf_dropout(ptr(x2), ld(x2), ptr(r2), ld(r2), ptr(y), cols, x2.size(0), cols, type_of(x), p,
-                      rng.const_data_ptr<int64_t>(), stream_of(x)),
+                      words(rng), stream_of(x)),
           "otf_dropout");
     return y;
 }
@@ -179,7 +180,7 @@ std::pair<Tensor, Tensor> add_norm_call(const Tensor& x, const Tensor& residual,
     Tensor y = at::empty(x.sizes(), x.options());
     Tensor z = at::empty(x.sizes(), residual.options());
     check(otf_dropout_add_layer_norm(ptr(x2), ld(x2), type_of(x), ptr(r2), ld(r2), type_of(residual), ptr(w), ptr(b),
-                                     param_type(weight, bias), eps, p, rng.const_data_ptr<int64_t>(), x2.size(0), cols,
+                                     param_type(weight, bias), eps, p, words(rng), x2.size(0), cols,
                                      ptr(y), cols, ptr(z), cols, stat(stats, 0), stat(stats, 1), stream_of(x)),
           "otf_dropout_add_layer_norm");
     return {y, z};
@@ -187,8 +188,9 @@ std::pair<Tensor, Tensor> add_norm_call(const Tensor& x, const Tensor& residual,
 
 struct AddNorm : torch::autograd::Function<AddNorm> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& residual, const OptTensor& weight,
-                                 const OptTensor& bias, double p, const Tensor& rng, double eps) {
+                                 const OptTensor& bias, double p, const OptTensor& state, double eps) {
         const c10::DeviceGuard guard(x.device());
+        const Tensor rng = value(state);
         const int64_t cols = x.size(-1);
         const Tensor x2 = rows_of(x, cols), r2 = rows_of(residual, cols), stats = stats_of(x2.size(0), x);
         auto [y, z] = add_norm_call(x, residual, weight, bias, p, rng, eps, x2, r2, stats);
@@ -230,7 +232,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         check(otf_dropout_add_layer_norm_backward(ptr(dy2), ld(dy2), ptr(dz2), ld(dz2), ptr(z2), ld(z2), ptr(x2), ld(x2),
                                                   ptr(r2), ld(r2), type_of(dx), type_of(dr), ptr(w), type, stat(stats, 0),
                                                   stat(stats, 1), ctx->saved_data["p"].toDouble(),
-                                                  rng.const_data_ptr<int64_t>(), rows, cols, ptr(dx), cols, ptr(dr), cols,
+                                                  words(rng), rows, cols, ptr(dx), cols, ptr(dr), cols,
                                                   ptr(g.dw), ptr(g.db), ptr(g.ws), bytes_of(g.ws), stream_of(stats)),
               "otf_dropout_add_layer_norm_backward");
         return once({ctx->saved_data["x"].toBool() ? dx : Tensor(), ctx->saved_data["residual"].toBool() ? dr : Tensor(),
@@ -239,14 +241,14 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
 };
 
 std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
-                                                 const OptTensor& bias, double p, const Tensor& rng, double eps) {
+                                                 const OptTensor& bias, double p, const OptTensor& rng, double eps) {
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(weight) || wants(bias))) {
         const variable_list o = AddNorm::apply(x, residual, weight, bias, p, rng, eps);
         return {o[0], o[1]};
     }
     const c10::DeviceGuard guard(x.device());
     const int64_t cols = x.size(-1);
-    return add_norm_call(x, residual, weight, bias, p, rng, eps, rows_of(x, cols), rows_of(residual, cols), Tensor());
+    return add_norm_call(x, residual, weight, bias, p, value(rng), eps, rows_of(x, cols), rows_of(residual, cols), Tensor());
 }
 
 // -------------------------------------------------------------------- gated feed-forward

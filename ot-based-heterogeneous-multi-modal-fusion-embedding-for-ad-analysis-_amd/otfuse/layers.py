@@ -155,11 +155,10 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torc
         raise TypeError(f"residual must have x's type ({x.dtype}) or float32, not {residual.dtype}")
     _norm_params(x, weight, bias)
     p, eps = _probability(p), _eps(eps)
-    if rng is None:
-        if p:
-            raise ValueError("p > 0 needs rng (rng_state)")
-        rng = torch.zeros(2, dtype=torch.int64, device=x.device)
-    return _native().dropout_add_layer_norm(x, residual, weight, bias, p, _rng(rng, x), eps)
+    if rng is None and p:
+        raise ValueError("p > 0 needs rng (rng_state)")
+    rng = None if rng is None else _rng(rng, x)
+    return _native().dropout_add_layer_norm(x, residual, weight, bias, p, rng, eps)
 
 
 # ------------------------------------------------------------------ gated feed-forward

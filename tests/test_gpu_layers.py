@@ -132,7 +132,7 @@ def test_dropout_backward_notices_a_changed_state(dev):
 
 
 # -------------------------------------------------------------------------- layer norm
-NORMS = [(1, 1), (3, 8), (70, 33), (129, 512), (9, 1000), (40, 1531), (17, 2048), (6, 4096), (33, 4100), (5, 8192),
+NORMS = [(5, 5), (1000, 100), (257, 128), (2000, 65), (901, 200), (333, 256), (10, 16384), (6, 16400), (1, 1), (3, 8), (70, 33), (129, 512), (9, 1000), (40, 1531), (17, 2048), (6, 4096), (33, 4100), (5, 8192),
          (3, 12345), (2, 32768), (2, 40001), (700, 64), (3000, 24)]
 
 
@@ -237,7 +237,7 @@ def test_layer_norm_empty_and_refusals(dev):
 
 @pytest.mark.parametrize("dt,rt", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f16", "f16")])
 @pytest.mark.parametrize("rows,cols,p", [(1, 1, 0.0), (8, 2048, 0.1), (70, 333, 0.3), (12, 4096, 0.5), (3, 9000, 0.1),
-                                        (2, 20000, 0.1), (2, 33001, 0.2), (600, 48, 0.1)])
+                                        (2, 20000, 0.1), (2, 33001, 0.2), (600, 48, 0.1), (100, 120, 0.2), (77, 250, 0.0), (30, 1500, 0.1)])
 def test_dropout_add_layer_norm(dev, dt, rt, rows, cols, p):
     from otfuse import layers
     seed, offset = 77 + rows, 5
@@ -267,6 +267,10 @@ def test_dropout_add_layer_norm(dev, dt, rt, rows, cols, p):
     _within(grads[1], g, tg + half(T[rt]) * g.abs())
     _within(grads[2], dw, tw)
     _within(grads[3], db, tb)
+    if p == 0:   # no state needed
+        y0, z0 = layers.dropout_add_layer_norm(x, res, w, b)
+        assert torch.equal(y0, y) and torch.equal(z0, z)
+        assert all(torch.equal(g0, g1) for g0, g1 in zip(torch.autograd.grad((y0, z0), (x, res, w, b), (dy, dz)), grads))
     # either output alone
     only = torch.autograd.grad(z, (x, res), dz, retain_graph=True)
     _within(only[1], dzd, half(T[rt]) * dzd.abs())

@@ -77,6 +77,7 @@ def test_dropout_refuses(clib):
         assert call(**kw) == L.OTF_EINVAL, kw
     assert call(cols=2 ** 31, ldx=2 ** 31, ldy=2 ** 31) == L.OTF_EUNSUPPORTED
     assert call(rows=0, x=None, y=None) == L.OTF_OK and call(cols=0) == L.OTF_OK
+    assert call(p=2.0 ** -17, rng=None) == L.OTF_EINVAL   # rounds to 2^-16: needs the state
 
 
 def test_layer_norm_refuses(clib):
@@ -139,6 +140,7 @@ def test_gated_ffn_refuses(clib):
     assert need >= 20 * 24 * 2   # h
     assert fwd(saved=None, ws=None) == L.OTF_EINVAL and fwd(saved=None, size=need - 1) == L.OTF_EINVAL
     assert fwd(d=(1 << 20) + 1) == L.OTF_EUNSUPPORTED and fwd(rows=1 << 30) == L.OTF_EUNSUPPORTED
+    assert fwd(d=1 << 18, f=1 << 18) == L.OTF_EUNSUPPORTED and fwd(rows=1 << 26, f=1 << 12) == L.OTF_EUNSUPPORTED
     assert fwd(rows=0, x=None) == L.OTF_OK
     for kw in (dict(dy=None), dict(saved=None), dict(w_down=None), dict(w_up=None), dict(dw_up=None), dict(dw_gate=None),
                dict(lddy=15), dict(lddx=15), dict(lddw_in=15), dict(lddw_down=23), dict(x=None), dict(dx=P + 1),
