@@ -1,10 +1,11 @@
 // otf_torch.cpp — the fusion block's layers as autograd nodes over the C ABI (include/otfuse.h).
 //
-// otfuse/layers.py checks the arguments; this module allocates the results, calls libotfuse.so on
-// the current stream of the tensors' device, and records backward.  Native rather than Python
-// because the layers' smallest calls are bound by the host: a trained dropout of 8 x 512 float32
-// took 107 us as a torch.autograd.Function in Python, whose backward has to take the interpreter
-// lock on the engine's thread, against 6 us of kernels.
+// This module checks the arguments of otfuse/layers.py's functions, allocates the results, calls
+// libotfuse.so on the current stream of the tensors' device, and records backward.  Native rather
+// than Python because the layers' smallest calls are bound by the host: a trained dropout of 8 x 512
+// float32 took 107 us as a torch.autograd.Function in Python, whose backward has to take the
+// interpreter lock on the engine's thread, against 4 us of kernels (47 us here); a norm of one token
+// 16 us, 7 with the checks in Python.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -55,6 +56,52 @@ const int64_t* words(const Tensor& rng) { return rng.defined() ? rng.const_data_
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && wants(*t); }
 
+// ---- what every entry point refuses (TypeError, ValueError) --------------------------------
+std::string text(const Tensor& t) {
+    std::ostringstream o;
+    o << t.sizes() << " " << t.scalar_type();
+    return o.str();
+}
+void input(const Tensor& t, const char* name) {
+    if (!t.defined() || !t.is_cuda()) throw py::type_error(std::string(name) + " must be a ROCm device tensor");
+    const auto k = t.scalar_type();
+    if (k != at::kFloat && k != at::kHalf && k != at::kBFloat16)
+        throw py::type_error(std::string(name) + ": float32, bfloat16 or float16, not " + text(t));
+}
+void beside(const Tensor& x, const Tensor& t, const char* name) {
+    if (t.device() != x.device()) throw py::value_error(std::string(name) + " is not on x's device");
+}
+double probability(double p) {
+    if (!(p >= 0.0 && p <= 1.0)) throw py::value_error("dropout probability " + std::to_string(p) + " is not in [0, 1]");
+    return p;
+}
+double epsilon(double eps) {
+    if (!(eps >= 0.0 && eps < std::numeric_limits<double>::infinity()))
+        throw py::value_error("eps " + std::to_string(eps) + " must be finite and not negative");
+    return eps;
+}
+void state(const Tensor& rng, const Tensor& x) {
+    if (rng.scalar_type() != at::kLong || rng.dim() != 1 || rng.size(0) != 2 || !rng.is_contiguous())
+        throw py::type_error("rng must be a contiguous int64 tensor [seed, offset] (rng_state)");
+    beside(x, rng, "rng");
+}
+void norm_params(const Tensor& x, const OptTensor& weight, const OptTensor& bias) {
+    if (x.dim() == 0 || x.size(-1) == 0) throw py::value_error("x " + text(x) + ": layer norm needs a last dimension of at least 1");
+    const OptTensor* both[2] = {&weight, &bias};
+    for (int i = 0; i < 2; ++i) {
+        if (!both[i]->has_value()) continue;
+        const Tensor& t = **both[i];
+        const char* name = i ? "bias" : "weight";
+        input(t, name);
+        beside(x, t, name);
+        if (t.dim() != 1 || t.size(0) != x.size(-1)) throw py::value_error(std::string(name) + " " + text(t) + " must have x's columns");
+        if (t.scalar_type() != x.scalar_type() && t.scalar_type() != at::kFloat)
+            throw py::type_error(std::string(name) + " must have x's type or float32, not " + text(t));
+    }
+    if (weight.has_value() && bias.has_value() && weight->scalar_type() != bias->scalar_type())
+        throw py::type_error("weight and bias must share one type");
+}
+
 // Gradients of kernels are not differentiable: under create_graph they carry a node that says so
 // when it is reached.
 variable_list once(variable_list grads) {
@@ -95,7 +142,16 @@ struct Dropout : torch::autograd::Function<Dropout> {
     }
 };
 
-Tensor dropout(const Tensor& x, const OptTensor& residual, double p, const Tensor& rng) {
+Tensor dropout(const Tensor& x, double p, const Tensor& rng, const OptTensor& residual) {
+    input(x, "x");
+    if (residual.has_value()) {
+        input(*residual, "residual");
+        beside(x, *residual, "residual");
+        if (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type())
+            throw py::value_error("residual " + text(*residual) + " differs from x " + text(x));
+    }
+    probability(p);
+    state(rng, x);
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual))) return Dropout::apply(x, residual, p, rng);
     return dropout_call(x, value(residual), p, rng);
 }
@@ -165,6 +221,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    input(x, "x");
+    norm_params(x, weight, bias);
+    epsilon(eps);
     if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias)))
         return LayerNorm::apply(x, weight, bias, eps);
     const c10::DeviceGuard guard(x.device());
@@ -242,6 +301,19 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
 
 std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                                  const OptTensor& bias, double p, const OptTensor& rng, double eps) {
+    input(x, "x");
+    input(residual, "residual");
+    beside(x, residual, "residual");
+    if (residual.sizes() != x.sizes()) throw py::value_error("residual " + text(residual) + " differs from x " + text(x));
+    if (residual.scalar_type() != x.scalar_type() && residual.scalar_type() != at::kFloat)
+        throw py::type_error("residual must have x's type or float32, not " + text(residual));
+    norm_params(x, weight, bias);
+    probability(p);
+    epsilon(eps);
+    if (rng.has_value())
+        state(*rng, x);
+    else if (p > 0.0)
+        throw py::value_error("p > 0 needs rng (rng_state)");
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual) || wants(weight) || wants(bias))) {
         const variable_list o = AddNorm::apply(x, residual, weight, bias, p, rng, eps);
         return {o[0], o[1]};
@@ -318,7 +390,22 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
     }
 };
 
-Tensor gated_feed_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, int64_t act) {
+Tensor gated_feed_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const std::string& activation) {
+    input(x, "x");
+    const std::pair<const Tensor*, const char*> weights[3] = {{&wg, "w_gate"}, {&wu, "w_up"}, {&wd, "w_down"}};
+    for (const auto& [t, name] : weights) {
+        input(*t, name);
+        beside(x, *t, name);
+        if (t->scalar_type() != x.scalar_type()) throw py::type_error(std::string(name) + " " + text(*t) + " must have x's type");
+    }
+    const int64_t act = activation == "silu" ? OTF_ACT_SILU : activation == "gelu" ? OTF_ACT_GELU : -1;
+    if (act < 0) throw py::value_error("activation '" + activation + "': silu or gelu");
+    const int64_t d = x.dim() ? x.size(-1) : 0;
+    if (wg.dim() != 2 || wg.size(1) != d || wu.sizes() != wg.sizes() || wd.dim() != 2 || wd.size(0) != d || wd.size(1) != wg.size(0))
+        throw py::value_error("x " + text(x) + ", w_gate " + text(wg) + ", w_up " + text(wu) + " and w_down " + text(wd) +
+                              " must be (..., d), (f, d), (f, d) and (d, f)");
+    if (d == 0 || wg.size(0) == 0 || std::max(d, wg.size(0)) > kMaxLd)
+        throw py::value_error("widths d = " + std::to_string(d) + " and f = " + std::to_string(wg.size(0)) + " must be between 1 and 2^20");
     if (at::GradMode::is_enabled() && (wants(x) || wants(wg) || wants(wu) || wants(wd)))
         return GatedFeedForward::apply(x, wg, wu, wd, act);
     return ffn_call(x, wg, wu, wd, act, nullptr);

@@ -30,7 +30,6 @@ COMM_ID_BYTES = 128
 SK_RUNNING, SK_CONVERGED, SK_MAX_ITER, SK_NUMERICAL_BREAK, SK_TIMEOUT = 0, 1, 2, 3, 4
 STATUS_NAMES = {0: "running", 1: "converged", 2: "max_iter", 3: "numerical_break",
                 4: "timeout"}
-ACTIVATIONS = {"silu": 0, "gelu": 1}
 ENGINE_AUTO, ENGINE_STREAM, ENGINE_RESIDENT, ENGINE_TILED, ENGINE_SWEEP, ENGINE_GATHER, ENGINE_MESH = (
     0, 1, 2, 3, 4, 5, 6)
 ENGINES = {"auto": ENGINE_AUTO, "stream": ENGINE_STREAM, "resident": ENGINE_RESIDENT,

@@ -24,7 +24,6 @@ import os
 import torch
 
 from . import _lib as L
-from .ops import _EMB_DT
 
 NODES_PATH = os.path.join(os.path.dirname(L.LIB_PATH), "_otf_layers.so")
 _nodes = None
@@ -45,27 +44,6 @@ def _native():
     return _nodes
 
 
-def _input(t, name: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a ROCm device tensor")
-    if t.dtype not in _EMB_DT:
-        raise TypeError(f"{name}: float32, bfloat16 or float16, not {t.dtype}")
-    return t
-
-
-def _same_device(ref: torch.Tensor, **others):
-    for name, t in others.items():
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{name} is on {t.device}, x on {ref.device}")
-
-
-def _probability(p) -> float:
-    p = float(p)
-    if not 0.0 <= p <= 1.0:
-        raise ValueError(f"dropout probability {p} is not in [0, 1]")
-    return p
-
-
 def rng_state(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
     """The generator's state as the layers take it: a device int64 tensor ``[seed, offset]``.
 
@@ -77,13 +55,6 @@ def rng_state(seed: int, offset: int = 0, device="cuda") -> torch.Tensor:
     return torch.tensor([seed, offset], dtype=torch.int64, device=device)
 
 
-def _rng(rng, x) -> torch.Tensor:
-    if not isinstance(rng, torch.Tensor) or rng.dtype != torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
-        raise TypeError("rng must be a contiguous int64 tensor [seed, offset] (rng_state)")
-    _same_device(x, rng=rng)
-    return rng
-
-
 # ----------------------------------------------------------------------------- dropout
 def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
     """``[residual +] dropout(x)`` (``--projection-dropout``).
@@ -92,40 +63,10 @@ def dropout(x: torch.Tensor, p: float, rng: torch.Tensor, residual: torch.Tensor
     scaled by its inverse; a dropped one is exactly 0, whatever it held.  The mask comes from
     ``rng`` (see ``rng_state``) and the element's row and column and is made again in backward
     instead of being stored.  x: (..., cols); residual: the same shape and type."""
-    _input(x, "x")
-    if residual is not None:
-        _input(residual, "residual")
-        _same_device(x, residual=residual)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual {tuple(residual.shape)} {residual.dtype} differs from x {tuple(x.shape)} {x.dtype}")
-    return _native().dropout(x, residual, _probability(p), _rng(rng, x))
+    return _native().dropout(x, p, rng, residual)
 
 
 # -------------------------------------------------------------------------- layer norm
-def _norm_params(x, weight, bias):
-    cols = x.shape[-1] if x.dim() else 0
-    if cols == 0:
-        raise ValueError(f"x {tuple(x.shape)}: layer norm needs a last dimension of at least 1")
-    kind = None
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        _input(t, name)
-        _same_device(x, **{name: t})
-        if t.shape != (cols,):
-            raise ValueError(f"{name} {tuple(t.shape)} must be ({cols},)")
-        if t.dtype not in (x.dtype, torch.float32) or kind not in (None, t.dtype):
-            raise TypeError(f"weight and bias must share one type, x's ({x.dtype}) or float32")
-        kind = t.dtype
-
-
-def _eps(eps) -> float:
-    eps = float(eps)
-    if not 0.0 <= eps < float("inf"):
-        raise ValueError(f"eps {eps} must be finite and not negative")
-    return eps
-
-
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                eps: float = 1e-5) -> torch.Tensor:
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension
@@ -133,9 +74,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
     x: (..., cols); weight, bias: (cols,), of one type, x's or float32.  The gradients of
     weight and bias are sums in a fixed order: the same bits every call."""
-    _input(x, "x")
-    _norm_params(x, weight, bias)
-    return _native().layer_norm(x, weight, bias, _eps(eps))
+    return _native().layer_norm(x, weight, bias, eps)
 
 
 def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | None = None,
@@ -146,25 +85,10 @@ def dropout_add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: torc
     residual and z: x's type or float32 (a 32-bit residual stream under 16-bit layers); y: x's
     type, of the float32 sum.  ``rng`` may be None where ``p`` is 0.  Backward keeps a float32 z,
     else x and residual."""
-    _input(x, "x")
-    _input(residual, "residual")
-    _same_device(x, residual=residual)
-    if residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} differs from x {tuple(x.shape)}")
-    if residual.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"residual must have x's type ({x.dtype}) or float32, not {residual.dtype}")
-    _norm_params(x, weight, bias)
-    p, eps = _probability(p), _eps(eps)
-    if rng is None and p:
-        raise ValueError("p > 0 needs rng (rng_state)")
-    rng = None if rng is None else _rng(rng, x)
     return _native().dropout_add_layer_norm(x, residual, weight, bias, p, rng, eps)
 
 
 # ------------------------------------------------------------------ gated feed-forward
-_MAX_WIDTH = 1 << 20   # the kernels' row strides: 256 rows within a 31-bit byte offset
-
-
 def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                        activation: str = "silu") -> torch.Tensor:
     """``(act(x @ w_gate.T) * (x @ w_up.T)) @ w_down.T``: the gated form of the fusion block's
@@ -173,18 +97,4 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     x: (..., d); w_gate, w_up: (f, d); w_down: (d, f), as ``torch.nn.Linear`` keeps them, all of
     x's type.  ``activation``: "silu" or "gelu" (the exact form).  Sums are float32; the hidden
     activations are rounded to x's type, the two products that backward needs are kept in float32."""
-    _input(x, "x")
-    for name, t in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        _input(t, name)
-        _same_device(x, **{name: t})
-        if t.dtype != x.dtype:
-            raise TypeError(f"{name} is {t.dtype}, x is {x.dtype}")
-    if activation not in L.ACTIVATIONS:
-        raise ValueError(f"activation {activation!r}: one of {sorted(L.ACTIVATIONS)}")
-    d = x.shape[-1] if x.dim() else 0
-    if w_gate.dim() != 2 or w_gate.shape[1] != d or w_up.shape != w_gate.shape or w_down.shape != (d, w_gate.shape[0]):
-        raise ValueError(f"x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} and w_down "
-                         f"{tuple(w_down.shape)} must be (..., d), (f, d), (f, d) and (d, f)")
-    if d == 0 or w_gate.shape[0] == 0 or max(d, w_gate.shape[0]) > _MAX_WIDTH:
-        raise ValueError(f"widths d = {d} and f = {w_gate.shape[0]} must be between 1 and {_MAX_WIDTH}")
-    return _native().gated_feed_forward(x, w_gate, w_up, w_down, L.ACTIVATIONS[activation])
+    return _native().gated_feed_forward(x, w_gate, w_up, w_down, activation)
