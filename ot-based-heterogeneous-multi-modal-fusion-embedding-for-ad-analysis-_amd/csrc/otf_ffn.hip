@@ -351,7 +351,7 @@ template <typename T, int R> __device__ __forceinline__ uint32_t tr_address(cons
 // their way while the MFMAs of one run, one barrier a K-tile.  These tiles serve products that do
 // not fill the chip with large ones, whose K loop is bound by the latency of a load.
 template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int S, int EPI>
-__global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64 * WGM * WGN, TM == 64 ? 3 : 2) void ffn_gemm_kernel(GemmArgs a) {
     constexpr int NT = 64 * WGM * WGN, TH = TN / 2, RA = TM / WGM / 16, RB = TH / WGN / 16;
     using TA = Tile<T, TRA, TM, NT>;
     using TB = Tile<T, TRB, TH, NT>;
@@ -394,13 +394,18 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
         cb[1].template load<true>(tb, kt, dst + TA::BYTES + TB::BYTES);
     };
 
-    f32x4 acc[2][RB][RA];
+    // float32 operands: a sum for each half of the K-tiles, added at the end.  The rounding of a sum
+    // grows with the root of its length, and theirs is not hidden under a 16-bit result's.
+    constexpr int SUMS = sizeof(T) == 4 ? 2 : 1;
+    f32x4 acc[SUMS][2][RB][RA];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int c = 0; c < SUMS; ++c)
 #pragma unroll
-        for (int j = 0; j < RB; ++j)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < RA; ++i) acc[h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < RB; ++j)
+#pragma unroll
+                for (int i = 0; i < RA; ++i) acc[c][h][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     uint32_t xa[RA], xb[RB];   // layout T: addresses in the first buffer
 #pragma unroll
@@ -449,7 +454,8 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
                 for (int j = 0; j < RB; ++j)
 #pragma unroll
-                    for (int i = 0; i < RA; ++i) acc[h][j][i] = Frag<T>::mma(fb[h].f[j][s], fa.f[i][s], acc[h][j][i]);
+                    for (int i = 0; i < RA; ++i)
+                        acc[s % SUMS][h][j][i] = Frag<T>::mma(fb[h].f[j][s], fa.f[i][s], acc[s % SUMS][h][j][i]);
         // the reads have returned (the MFMAs used them) before this wave reaches the next barrier
         buf = buf + 1 == S ? 0 : buf + 1;
     }
@@ -460,7 +466,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
         for (int j = 0; j < RB; ++j) {
             const int m = m0 + (wm * RA + i) * 16 + (lane & 15), n = n0 + (wn * RB + j) * 16 + (lane >> 4) * 4;
-            finish4<T, EPI>(a, z, split, m, n, n + TH, acc[0][j][i], acc[1][j][i]);
+            f32x4 r0 = acc[0][0][j][i], r1 = acc[0][1][j][i];
+            if constexpr (SUMS == 2) r0 += acc[1][0][j][i], r1 += acc[1][1][j][i];
+            finish4<T, EPI>(a, z, split, m, n, n + TH, r0, r1);
         }
 }
 
