@@ -726,6 +726,65 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
     }
 }
 
+// ---- weight gradients of few rows -------------------------------------------------------------
+// C[r, c] = sum_n A[n, r] B[n, c] over up to NR rows, up to three such sums in one launch: bound by
+// the writing of C (bf16, 4096 x 11264, 1 to 8 rows: the three take 60 us where tiles take 120).  A
+// thread holds its 8 columns of B's rows in registers and walks `walk` rows of C, 16 or, where that
+// leaves CUs idle, 4; A's values come from LDS.
+struct OuterJob {
+    const void *a, *b;
+    void* c;
+    int64_t lda, ldb, ldc;
+    int R, C;
+    int across;     // threads across the columns, a power of two from 32 to 256
+    int wide;       // workgroups across the columns
+    int64_t first;  // the job's first workgroup
+};
+struct OuterArgs {
+    OuterJob job[3];
+    int count, rows, walk;
+};
+template <typename T, int NR> __global__ __launch_bounds__(256) void ffn_outer_kernel(OuterArgs o) {
+    __shared__ float sa[NR * 128];
+    int k = 0;
+    while (k + 1 < o.count && blockIdx.x >= o.job[k + 1].first) ++k;
+    const OuterJob& j = o.job[k];
+    const int block = (int)(blockIdx.x - j.first), deep = 256 / j.across, RB = o.walk * deep;
+    const int tx = threadIdx.x % j.across, ty = threadIdx.x / j.across;
+    const int r0 = (block / j.wide) * RB, col = ((block % j.wide) * j.across + tx) * 8;
+    for (int i = threadIdx.x; i < NR * RB; i += 256) {
+        const int n = i / RB, r = r0 + i % RB;
+        sa[i] = n < o.rows && r < j.R ? (float)((const T*)j.a)[n * j.lda + r] : 0.0f;
+    }
+    __syncthreads();
+    const int valid = j.C - col;
+    if (valid <= 0) return;
+    float b[NR][8];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+        if (n < o.rows) {
+            load8((const T*)j.b + n * j.ldb + col, valid, b[n]);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) b[n][q] = 0.0f;
+        }
+    }
+    for (int i = 0; i < o.walk; ++i) {
+        const int in = i * deep + ty, r = r0 + in;
+        if (r >= j.R) break;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+            const float a = sa[n * RB + in];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[q] += a * b[n][q];
+        }
+        store8((T*)j.c + (int64_t)r * j.ldc + col, valid, v);
+    }
+}
+
 // ---- copies for unaligned operands ---------------------------------------------------------
 // Rows copied to a leading dimension that is a multiple of 8, zeros past the last column.
 struct PackItem {
@@ -1013,6 +1072,38 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     return OTF_OK;
 }
 
+constexpr int kOuterRows = 16;
+
+// dWg, dWu and dWd, those that are wanted, of up to kOuterRows rows
+template <typename T>
+hipError_t run_outer(const Block& b, const char* dg, const char* du, const char* h, hipStream_t s) {
+    const otf_ffn_args* o = b.o;
+    OuterArgs args{};
+    args.rows = (int)b.n;
+    args.walk = b.d * b.f >= (int64_t)1 << 23 ? 16 : 4;   // 2^23: about 1024 workgroups of 16 rows by 256 threads
+    int64_t blocks = 0;
+    auto add = [&](const void* a, int64_t lda, int64_t R, const void* bb, int64_t ldb, int64_t C, void* c, int64_t ldc) {
+        int across = 32;
+        while (across < 256 && across * 8 < C) across *= 2;
+        const int64_t wide = (C + across * 8 - 1) / (across * 8), deep = args.walk * (256 / across);
+        args.job[args.count++] = OuterJob{a, bb, c, lda, ldb, ldc, (int)R, (int)C, across, (int)wide, blocks};
+        blocks += wide * ((R + deep - 1) / deep);
+    };
+    if (o->dw_gate) {
+        add(dg, b.fk, b.f, o->x, o->ldx, b.d, o->dw_gate, o->lddw_in);
+        add(du, b.fk, b.f, o->x, o->ldx, b.d, o->dw_up, o->lddw_in);
+    }
+    if (o->dw_down) add(o->dy, o->lddy, b.d, h, b.fk, b.f, o->dw_down, o->lddw_down);
+    if (!args.count) return hipSuccess;
+    if (b.n <= 4)
+        ffn_outer_kernel<T, 4><<<(unsigned)blocks, 256, 0, s>>>(args);
+    else if (b.n <= 8)
+        ffn_outer_kernel<T, 8><<<(unsigned)blocks, 256, 0, s>>>(args);
+    else
+        ffn_outer_kernel<T, kOuterRows><<<(unsigned)blocks, 256, 0, s>>>(args);
+    return hipGetLastError();
+}
+
 template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
     const Saved sv = carve_saved(o->saved, b.n, b.fk, b.es);
@@ -1022,7 +1113,8 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     b.operand(b.dy, o->dy, o->lddy, b.n, b.d);
     if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
     if (wx) b.weights_in();
-    if (win) b.operand(b.x, o->x, o->ldx, b.n, b.d);
+    const bool outer = b.n <= kOuterRows;   // the weights' gradients without tiles
+    if (win && !outer) b.operand(b.x, o->x, o->ldx, b.n, b.d);
     // dh = dy Wd: K = d, the rows of Wd
     Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.fk, nullptr, 0)};
     mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.fk;
@@ -1037,14 +1129,18 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     size_t slab = 0;   // one after another on the stream: they share it
     auto more = [&](const Product& p) { const size_t k = slab_bytes(p, plan_product(p, b.es)); slab = k > slab ? k : slab; };
     if (wx) more(px);
-    if (win) more(pi);
-    if (wdown) more(pd);
+    if (win && !outer) more(pi);
+    if (wdown && !outer) more(pd);
     float* part = (float*)b.ws.take(slab);
     *need = b.ws.used;
     if (!run) return OTF_OK;
     OTF_HIP(b.run_pack<T>(s));
     if (wx || win) OTF_HIP((launch_tiles<T, false, true, kGatedBackward>(mid.a, plan_product(mid, b.es), s)));
     if (wx) OTF_HIP((run_store<T, false, true>(px, part, s)));
+    if (outer) {
+        OTF_HIP((run_outer<T>(b, dg, du, sv.h, s)));
+        return OTF_OK;
+    }
     if (win) OTF_HIP((run_store<T, true, true>(pi, part, s)));
     if (wdown) OTF_HIP((run_store<T, true, true>(pd, part, s)));
     return OTF_OK;

@@ -27,6 +27,7 @@ namespace {
 // widest rows held in registers: 1024 threads x 4 chunks of 8; backward, which also holds the
 // parameter gradients' sums, 512 threads x 4
 constexpr int kMaxHeldCols = 32768, kMaxHeldColsBackward = 16384;
+constexpr int kFewRows = 64;   // up to here the parameter gradients share the backward launch
 
 struct NormArgs {
     const void* x;       // forward: input; backward: the normalised input (x or z), or with res x
@@ -292,26 +293,15 @@ __global__ __launch_bounds__(1024) void norm_forward_long_kernel(NormArgs a) {
     }
 }
 
-// One parameter gradient's partial sums, or (one workgroup) the gradient itself.
-template <typename T>
-__device__ __forceinline__ void store_param_grad(const NormArgs& a, int which, int col, const float (&s)[8]) {
-    const int valid = chunk_valid(a.cols, col);
-    if (gridDim.x == 1) {
-        void* out = which ? a.db : a.dw;
-        if (!out) return;
-        if (a.wf32)
-            store8((float*)out + col, valid, s);
-        else
-            store8((T*)out + col, valid, s);
-    } else {
-        store8(a.partial + ((int64_t)blockIdx.x * 2 + which) * a.cols + col, valid, s);
-    }
+// One parameter gradient's partial sums
+__device__ __forceinline__ void store_partial(const NormArgs& a, int which, int col, const float (&s)[8]) {
+    store8(a.partial + ((int64_t)blockIdx.x * 2 + which) * a.cols + col, chunk_valid(a.cols, col), s);
 }
 
-// Rows gridDim RPB apart.  WG: parameter gradients wanted.  TR: the type of residual and z (= T
+// Workgroup blockIdx.x of `groups`, its rows groups RPB apart.  WG: parameter gradients wanted.  TR: the type of residual and z (= T
 // without the residual sum); a 16-bit one makes the sum again from x and residual.
 template <typename T, typename TR, bool DROP, bool WG, int NT, int TPR, int CH>
-__global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
+__device__ __forceinline__ void norm_backward_rows(const NormArgs& a, int groups) {
     constexpr int RPB = NT / TPR;
     __shared__ float red[TPR > 64 ? 4 * (TPR / 64) : 1];
     __shared__ float comb[WG && RPB > 1 ? (NT / 64 - 1) * 64 * 8 : 1];
@@ -350,7 +340,7 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
         row_mean = a.mean[row];
         row_rstd = a.rstd[row];
     };
-    const int64_t first = (int64_t)blockIdx.x * RPB + part, step = (int64_t)gridDim.x * RPB;
+    const int64_t first = (int64_t)blockIdx.x * RPB + part, step = (int64_t)groups * RPB;
     if (AHEAD && first < a.rows) fetch(first);
     for (int64_t row = first; row < a.rows; row += step) {
         if (!AHEAD) fetch(row);
@@ -414,8 +404,8 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
             for (int c = 0; c < CH; ++c) {
                 const int col = (c * TPR + t) * 8;
                 if (col >= cols) continue;
-                store_param_grad<T>(a, 0, col, gw[c]);
-                store_param_grad<T>(a, 1, col, gb[c]);
+                store_partial(a, 0, col, gw[c]);
+                store_partial(a, 1, col, gb[c]);
             }
         } else {   // a wave's rows joined by exchanges, the waves through LDS, a chunk of one gradient at a time
             constexpr int NW = NT / 64;
@@ -439,7 +429,7 @@ __global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
                     for (int p = 0; p < NW - 1; ++p)
 #pragma unroll
                         for (int j = 0; j < 8; ++j) s[j] += comb[(p * 8 + j) * 64 + lane];
-                    store_param_grad<T>(a, i & 1, col, s);
+                    store_partial(a, i & 1, col, s);
                 }
             }
         }
@@ -512,19 +502,19 @@ __global__ __launch_bounds__(1024) void norm_backward_long_kernel(NormArgs a) {
     }
 }
 
-// Parameter gradients of rows wider than kMaxHeldColsBackward: 64 chunks of 8 columns by 4 waves;
-// the rows are dealt to gridDim.y workgroups and their waves in turn, one partial a workgroup.
-template <typename T, typename TR, bool DROP>
-__global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
-    __shared__ float comb[3 * 64 * 16];
+// Parameter gradients by columns: 64 chunks of 8 by the workgroup's NW waves, the rows dealt to
+// `parts` workgroups and their waves in turn; one partial a workgroup, or (parts = 1) the result.
+template <typename T, typename TR, bool DROP, int NW>
+__device__ __forceinline__ void norm_param_columns(const NormArgs& a, int block, int which, int parts) {
+    __shared__ float comb[(NW - 1) * 64 * 16];
     const int t = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t col = ((int64_t)blockIdx.x * 64 + t) * 8;
+    const int64_t col = ((int64_t)block * 64 + t) * 8;
     const int valid = col < a.cols ? (int)(a.cols - col < 8 ? a.cols - col : 8) : 0;
     float s[2][8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[0][j] = 0.0f, s[1][j] = 0.0f;
     if (valid > 0)
-        for (int64_t row = (int64_t)blockIdx.y * 4 + part; row < a.rows; row += (int64_t)gridDim.y * 4) {
+        for (int64_t row = (int64_t)which * NW + part; row < a.rows; row += (int64_t)parts * NW) {
             const float mean = a.mean[row], rstd = a.rstd[row];
             float v[8], g[8];
             load8((const TR*)a.x + row * a.ldx + col, valid, v);
@@ -543,11 +533,41 @@ __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
         for (int i = 0; i < 16; ++i) comb[((part - 1) * 16 + i) * 64 + t] = s[i >> 3][i & 7];
     __syncthreads();
     if (part > 0 || valid <= 0) return;
-    for (int p = 0; p < 3; ++p)
+    for (int p = 0; p < NW - 1; ++p)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[i >> 3][i & 7] += comb[(p * 16 + i) * 64 + t];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) store8(a.partial + ((int64_t)blockIdx.y * 2 + i) * a.cols + col, valid, s[i]);
+    for (int i = 0; i < 2; ++i) {
+        void* out = i ? a.db : a.dw;
+        if (parts > 1)
+            store8(a.partial + ((int64_t)which * 2 + i) * a.cols + col, valid, s[i]);
+        else if (out && a.wf32)
+            store8((float*)out + col, valid, s[i]);
+        else if (out)
+            store8((T*)out + col, valid, s[i]);
+    }
+}
+
+template <typename T, typename TR, bool DROP, bool WG, int NT, int TPR, int CH>
+__global__ __launch_bounds__(NT) void norm_backward_kernel(NormArgs a) {
+    norm_backward_rows<T, TR, DROP, WG, NT, TPR, CH>(a, gridDim.x);
+}
+
+// Few rows: the workgroups past `groups` take the parameter gradients, which need a row's statistics
+// but not its sums.  x and dy are read twice, from L2, and a second launch and its partials are
+// saved (8 x 2048 float32 with the autograd around it: 80 -> 75 us).
+template <typename T, typename TR, bool DROP, int NT, int TPR, int CH>
+__global__ __launch_bounds__(NT) void norm_backward_few_kernel(NormArgs a, int groups) {
+    if ((int)blockIdx.x < groups)
+        norm_backward_rows<T, TR, DROP, false, NT, TPR, CH>(a, groups);
+    else
+        norm_param_columns<T, TR, DROP, NT / 64>(a, blockIdx.x - groups, 0, 1);
+}
+
+// Rows wider than kMaxHeldColsBackward
+template <typename T, typename TR, bool DROP>
+__global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
+    norm_param_columns<T, TR, DROP, 4>(a, blockIdx.x, blockIdx.y, gridDim.y);
 }
 
 // partial [groups][2][cols] -> dw (blockIdx.y = 0), db (1).  64 columns a workgroup, its 16
@@ -624,7 +644,13 @@ template <typename T, typename TR, bool DROP, bool WG>
 hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
     const int c = a.cols, grid = norm_backward_groups(a.rows, c);
     const bool held = c <= kMaxHeldColsBackward;
-#define OTF_NB(NT, TPR, CH) norm_backward_kernel<T, TR, DROP, WG, NT, TPR, CH><<<grid, NT, 0, s>>>(a)
+    const bool few = WG && held && a.rows <= kFewRows;
+    const int columns = (c - 1) / 512 + 1;
+#define OTF_NB(NT, TPR, CH)                                                                                      \
+    if (few)                                                                                                     \
+        norm_backward_few_kernel<T, TR, DROP, NT, TPR, CH><<<grid + columns, NT, 0, s>>>(a, grid);               \
+    else                                                                                                         \
+        norm_backward_kernel<T, TR, DROP, WG, NT, TPR, CH><<<grid, NT, 0, s>>>(a)
     if (c <= 64) {
         OTF_NB(256, 8, 1);
     } else if (c <= 128) {
@@ -648,7 +674,7 @@ hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
         if (WG) norm_param_long_kernel<T, TR, DROP><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
     }
 #undef OTF_NB
-    if (WG && (grid > 1 || !held)) {
+    if (WG && !few && grid > 1) {
         const dim3 g((unsigned)((c + 63) / 64), 2);
         if (a.wf32)
             norm_param_kernel<float><<<g, 1024, 0, s>>>(a.partial, grid, c, (float*)a.dw, (float*)a.db);
@@ -786,8 +812,9 @@ int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const 
 
 size_t otf_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
+    if (cols <= kMaxHeldColsBackward && rows <= kFewRows) return 0;
     const int g = norm_backward_groups(rows, cols);
-    return g > 1 || cols > kMaxHeldColsBackward ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;
+    return g > 1 ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;
 }
 
 // shared by the two backward entry points

@@ -291,7 +291,7 @@ def _close(got, want, roundings, dtype, depth):
     assert excess <= 0, f"an element is {excess:.3e} beyond eight deviations"
 
 
-FFNS = [(9, 640, 48), (16, 48, 2100), (12, 1100, 600), (1, 8, 16), (1, 1, 1), (1, 1000, 333), (3, 64, 96), (16, 130, 100), (16, 512, 1032), (17, 72, 136), (33, 250, 71),
+FFNS = [(7, 2056, 4100), (14, 4104, 2050), (9, 640, 48), (16, 48, 2100), (12, 1100, 600), (1, 8, 16), (1, 1, 1), (1, 1000, 333), (3, 64, 96), (16, 130, 100), (16, 512, 1032), (17, 72, 136), (33, 250, 71),
         (64, 64, 64), (130, 512, 264), (200, 1000, 334), (257, 136, 1100), (5, 2048, 40), (700, 40, 2056), (513, 1024, 1408)]
 
 
