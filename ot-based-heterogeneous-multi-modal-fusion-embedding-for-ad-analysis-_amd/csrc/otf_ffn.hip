@@ -181,12 +181,12 @@ template <typename T, bool TR, int R, int NT> struct Tile {
 };
 
 // ---- results ------------------------------------------------------------------------------
-enum { kStore = 0, kPartial = 1, kGatedForward = 2, kGatedBackward = 3 };
+enum { kStore = 0, kGatedForward = 1, kGatedBackward = 2 };
 struct GemmArgs {
     Operand a, b;
     int M, N;            // extent of the result; gated forward: N = features
     int segments;        // of K (each a.k deep)
-    int splits;          // of the K-tiles, kPartial: one slab of C each
+    int splits;          // of the K-tiles, kStore: with more than one, c[0] is a float32 slab of C each
     int tiles_m, tiles_n;
     void* c[2];          // result; second: the rows past tiles of the first (batch), see batch
     int64_t ldc;         // elements
@@ -226,14 +226,16 @@ template <typename T, int EPI>
 __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int m, int n, int n2, f32x4 acc0, f32x4 acc1) {
     if (m >= a.M) return;
     if constexpr (EPI == kStore) {
+        if (a.splits > 1) {   // ldc: a multiple of 4 past N
+            float* c = (float*)a.c[0] + (((int64_t)split * a.batch + z) * a.M + m) * a.ldc;
+            if (n < a.N) *reinterpret_cast<f32x4*>(c + n) = acc0;
+            if (n2 < a.N) *reinterpret_cast<f32x4*>(c + n2) = acc1;
+            return;
+        }
         T* c = (T*)a.c[z] + (int64_t)m * a.ldc;
         const bool vec = (a.ldc & 3) == 0 && ((uintptr_t)a.c[z] & (4 * sizeof(T) - 1)) == 0;
         store4(c + n, a.N - n, vec, acc0);
         store4(c + n2, a.N - n2, vec, acc1);
-    } else if constexpr (EPI == kPartial) {   // ldc: a multiple of 4 past N
-        float* c = (float*)a.c[0] + (((int64_t)split * a.batch + z) * a.M + m) * a.ldc;
-        if (n < a.N) *reinterpret_cast<f32x4*>(c + n) = acc0;
-        if (n2 < a.N) *reinterpret_cast<f32x4*>(c + n2) = acc1;
     } else if constexpr (EPI == kGatedForward) {
         if (n >= a.N) return;   // N, ldh whole K-tiles
         const int64_t o = (int64_t)m * a.ldh + n;
@@ -350,19 +352,20 @@ template <typename T, int R> __device__ __forceinline__ uint32_t tr_address(cons
 // TM x TN tile (B in two halves of TN / 2), WGM x WGN waves.  S buffers of one K-tile: S - 1 are on
 // their way while the MFMAs of one run, one barrier a K-tile.  These tiles serve products that do
 // not fill the chip with large ones, whose K loop is bound by the latency of a load.
+// gemm_tile: tile `id` of product z, slab `split`; smem: S (TM + TN) K-tiles' rows.
 template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int S, int EPI>
-__global__ __launch_bounds__(64 * WGM * WGN, TM == 64 ? 3 : 2) void ffn_gemm_kernel(GemmArgs a) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, int z, int split, char* smem) {
     constexpr int NT = 64 * WGM * WGN, TH = TN / 2, RA = TM / WGM / 16, RB = TH / WGN / 16;
     using TA = Tile<T, TRA, TM, NT>;
     using TB = Tile<T, TRB, TH, NT>;
     constexpr int BUF = TA::BYTES + 2 * TB::BYTES;
     constexpr int LOADS = TA::PER + 2 * TB::PER;   // a wave's, a K-tile
-    __shared__ __attribute__((aligned(16))) char smem[S * BUF];
+    static_assert(BUF == (TM + TN) * kTileBytes, "what the callers set aside");
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid / WGN, wn = wid % WGN;
 
-    const int tiles = a.tiles_m * a.tiles_n, z = blockIdx.y % a.batch, split = blockIdx.y / a.batch;
+    const int tiles = a.tiles_m * a.tiles_n;
     int tm, tn;
-    tile_of(blockIdx.x, tiles, a.tiles_m, a.tiles_n, tm, tn);
+    tile_of(id, tiles, a.tiles_m, a.tiles_n, tm, tn);
     const int m0 = tm * TM, n0 = EPI == kGatedForward ? tn * TH : tn * TN;
 
     TA ta;
@@ -472,26 +475,33 @@ __global__ __launch_bounds__(64 * WGM * WGN, TM == 64 ? 3 : 2) void ffn_gemm_ker
         }
 }
 
+template <typename T, bool TRA, bool TRB, int TM, int TN, int WGM, int WGN, int S, int EPI>
+__global__ __launch_bounds__(64 * WGM * WGN, TM == 64 ? 3 : 2) void ffn_gemm_kernel(GemmArgs a) {
+    __shared__ __attribute__((aligned(16))) char smem[S * (TM + TN) * kTileBytes];
+    gemm_tile<T, TRA, TRB, TM, TN, WGM, WGN, S, EPI>(a, blockIdx.x, blockIdx.y % a.batch, blockIdx.y / a.batch, smem);
+}
+
 // ---- the tiled product, 256 x 256 -----------------------------------------------------------
-// 16-bit operands, whole K-tiles where an operand is K-contiguous, eight waves in 2 (m) x 4 (n), each 2 x 64 rows by 2 x 32 columns: 128
-// accumulator registers a lane.  Each operand's tile is two half-tiles of 16 KB; two K-tiles of
+// 16-bit operands, whole K-tiles where an operand is K-contiguous, eight waves in 2 (m) x 4 (n),
+// each 2 x 64 rows by 2 x 32 columns: 128 accumulator registers a lane.  Each operand's tile is two half-tiles of 16 KB; two K-tiles of
 // four half-tiles fill 128 KB of LDS.  A K-tile runs as four phases, one quadrant of the result
 // each (A0 B0, A0 B1, A1 B1, A1 B0; B's halves the other way round in every second K-tile), so a
 // phase reads only the fragments that the registers do not hold, 8, 4, 8 and 4 of them.  Each
 // phase puts one half-tile in flight, up to two K-tiles ahead.  The two wave groups (m) run one
 // barrier apart, so on every SIMD one wave's MFMAs cover the other's LDS reads and loads.
+constexpr int kTile256Bytes = 2 * 4 * 128 * kTileBytes;
+// tile `id` of product z, slab `split`
 template <typename T, bool TRA, bool TRB, int EPI>
-__global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
+__device__ __forceinline__ void gemm256_tile(const GemmArgs& a, int id, int z, int split, char* smem) {
     static_assert(sizeof(T) == 2, "16-bit operands");
     constexpr int HT = 128 * kTileBytes, BUF = 4 * HT;   // half-tiles A0, A1, B0, B1
     using TA = Tile<T, TRA, 128, 512>;
     using TB = Tile<T, TRB, 128, 512>;
-    __shared__ __attribute__((aligned(16))) char smem[2 * BUF];
     const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, wm = wid >> 2, wn = wid & 3;
 
-    const int tiles = a.tiles_m * a.tiles_n, z = blockIdx.y % a.batch, split = blockIdx.y / a.batch;
+    const int tiles = a.tiles_m * a.tiles_n;
     int tm, tn;
-    tile_of(blockIdx.x, tiles, a.tiles_m, a.tiles_n, tm, tn);
+    tile_of(id, tiles, a.tiles_m, a.tiles_n, tm, tn);
     const int m0 = tm * 256, n0 = EPI == kGatedForward ? tn * 128 : tn * 256;
 
     TA ta;
@@ -621,6 +631,39 @@ __global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
                 const int m = m0 + h * 128 + wm * 64 + t * 16 + (lane & 15), n = n0 + wn * 32 + u * 16 + (lane >> 4) * 4;
                 finish4<T, EPI>(a, z, split, m, n, n + 128, acc[h][0][t][u], acc[h][1][t][u]);
             }
+}
+
+template <typename T, bool TRA, bool TRB, int EPI>
+__global__ __launch_bounds__(512) void ffn_gemm256_kernel(GemmArgs a) {
+    __shared__ __attribute__((aligned(16))) char smem[kTile256Bytes];
+    gemm256_tile<T, TRA, TRB, EPI>(a, blockIdx.x, blockIdx.y % a.batch, blockIdx.y / a.batch, smem);
+}
+
+// ---- two products in one launch -------------------------------------------------------------
+// Products that need nothing of each other, a's workgroups before b's: b's fill the CUs that a's
+// last round leaves and those that are done early, and a launch is saved (777 x 1000 x 2730 trained
+// 141 -> 126 us, 100 x 512 x 1408 42 -> 36).  Tiles of both side by side would share an L2 with the
+// other's operands: 8192 x 4096 x 11264, dWd and dh 1590-1630 us, an XCD of each kind in turn 1500,
+// one after the other 1370-1400, as two launches 1580.  Ids are counted in eights, so all keep their
+// XCDs.  B is row-contiguous in every product of backward.
+template <typename T, int SIDE, bool TRA, int EPI>
+__device__ __forceinline__ void pair_tile(const GemmArgs& g, int id, char* smem) {
+    const int tiles = g.tiles_m * g.tiles_n, each = (tiles + 7) / 8 * 8, y = id / each;
+    id -= y * each;
+    if (id >= tiles) return;
+    if constexpr (SIDE == 256)
+        gemm256_tile<T, TRA, true, EPI>(g, id, y % g.batch, y / g.batch, smem);
+    else
+        gemm_tile<T, TRA, true, SIDE, SIDE, 2, 2, SIDE == 64 ? 3 : 2, EPI>(g, id, y % g.batch, y / g.batch, smem);
+}
+template <typename T, int SIDE, bool TRA1, int EPI1, bool TRA2, int EPI2>
+__global__ __launch_bounds__(SIDE == 256 ? 512 : 256, SIDE == 64 ? 3 : 2) void ffn_gemm_pair_kernel(GemmArgs a, GemmArgs b, int first) {
+    __shared__ __attribute__((aligned(16))) char smem[(SIDE == 64 ? 3 : 2) * 2 * SIDE * kTileBytes];
+    const int id = blockIdx.x;
+    if (id < first)
+        pair_tile<T, SIDE, TRA1, EPI1>(a, id, smem);
+    else
+        pair_tile<T, SIDE, TRA2, EPI2>(b, id - first, smem);
 }
 
 // slabs [splits][batch][M][ldp] added in order and rounded once
@@ -840,8 +883,8 @@ struct Product {
 constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 
 // Tile side and slabs of K, by the least estimated time.  A CU holds one tile of 256, two of 128,
-// three of 64 or five of 16 by 64; a K-tile then takes it c microseconds (less where it holds fewer), a tile's start and
-// results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted to bf16 products of 64 to
+// three of 64 or five of 16 by 64; a K-tile then takes it c microseconds (less where it holds
+// fewer), a tile's start and results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted to bf16 products of 64 to
 // 4096 rows by 512 to 4096 and 1408 to 11264 columns, each run with all three sides:
 //   gate and up 1024 x 2048 x 5632   62 / 91 / 85 us with 256 / 128 / 64   (176, 704, 2816 tiles)
 //               64 x 4096 x 11264    85 / 93 / 58                          (88, 176, 352)
@@ -851,35 +894,93 @@ constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 struct Plan {
     int side, splits;
 };
-Plan plan_product(const Product& p, int elem) {
-    const GemmArgs& a = p.a;
-    const bool whole = elem == 2 && (p.tra || a.a.k % 64 == 0) && (p.trb || a.b.k % 64 == 0);
+int per_cu(int side) { return side == 256 ? 1 : side == 128 ? 2 : side == 64 ? 3 : 5; }
+int64_t tiles_of(const Product& p, int side) {
+    const int64_t across = side == 16 ? 64 : side, width = p.epi == kGatedForward ? across / 2 : across;
+    return (p.a.M + side - 1) / side * ((p.a.N + width - 1) / width) * p.a.batch;
+}
+int64_t ktiles_of(const Product& p, int elem) {
     const int depth = kTileBytes / elem;
-    const int64_t ktiles = (int64_t)((a.a.k + depth - 1) / depth) * a.segments;
+    return (int64_t)((p.a.a.k + depth - 1) / depth) * p.a.segments;
+}
+bool can_take(const Product& p, int elem, int side) {
+    if (side == 16) return !p.tra && p.a.M <= 16;
+    return side != 256 || (elem == 2 && (p.tra || p.a.a.k % 64 == 0) && (p.trb || p.a.b.k % 64 == 0));
+}
+// a tile of this many K-tiles where the launch fills `full` of the chip's slots
+double tile_us(int side, int elem, int64_t ktiles, double full) {
+    const double c = elem == 2 ? (side == 256 ? 1.35 : side == 128 ? 1.1 : side == 64 ? 0.75 : 0.6) : (side == 128 ? 4.2 : side == 64 ? 1.9 : 0.8);
+    const double e = side == 256 ? 14.0 : side == 128 ? 11.0 : 5.0;
+    return (double)ktiles * c * (side == 256 ? 1.0 : 0.5 + 0.5 * (full < 1.0 ? full : 1.0)) + e;
+}
+double join_us(const Product& p, int splits) {
+    return splits > 1 ? 4.0 + (double)splits * p.a.batch * p.a.M * p.a.N * 4.0 * (1 / 6.4e6 + 1 / 4.0e6) : 0.0;
+}
+Plan plan_product(const Product& p, int elem, double* us = nullptr) {
+    const int64_t ktiles = ktiles_of(p, elem);
     Plan best{64, 1};
     double least = 1e30;
     for (int side : {256, 128, 64, 16}) {   // 16: 16 rows by 64 columns
-        if ((side == 256 && !whole) || (side == 16 && (p.tra || a.M > 16))) continue;
-        const int per_cu = side == 256 ? 1 : side == 128 ? 2 : side == 64 ? 3 : 5;
-        const double c = elem == 2 ? (side == 256 ? 1.35 : side == 128 ? 1.1 : side == 64 ? 0.75 : 0.6) : (side == 128 ? 4.2 : side == 64 ? 1.9 : 0.8);
-        const double e = side == 256 ? 14.0 : side == 128 ? 11.0 : 5.0;
-        const int64_t across = side == 16 ? 64 : side, width = p.epi == kGatedForward ? across / 2 : across;
-        const int64_t rows = (a.M + side - 1) / side;
-        const int64_t tiles = rows * ((a.N + width - 1) / width) * a.batch, slots = (int64_t)kCus * per_cu;
+        if (!can_take(p, elem, side)) continue;
+        const int64_t tiles = tiles_of(p, side), slots = (int64_t)kCus * per_cu(side);
         for (int splits = 1; splits <= 32; splits *= 2) {
             if (splits > 1 && (p.epi != kStore || tiles * splits > slots || ktiles / splits < 4)) break;
             const double full = (double)(tiles * splits) / slots;
             const double rounds = full < 1.0 ? 1.0 : side <= 64 ? full : (double)((tiles + slots - 1) / slots);
-            const double speed = per_cu == 1 ? 1.0 : 0.5 + 0.5 * (full < 1.0 ? full : 1.0);
-            double us = rounds * ((double)((ktiles + splits - 1) / splits) * c * speed + e);
-            if (splits > 1) us += 4.0 + (double)splits * a.batch * a.M * a.N * 4.0 * (1 / 6.4e6 + 1 / 4.0e6);
-            if (us < least) least = us, best = Plan{side, splits};
+            const double t = rounds * tile_us(side, elem, (ktiles + splits - 1) / splits, full) + join_us(p, splits);
+            if (t < least) least = t, best = Plan{side, splits};
+        }
+    }
+    if (us) *us = least;
+    return best;
+}
+
+// na tiles of ta, then nb of tb, each where a slot is free first
+double two_runs_us(int64_t slots, int64_t na, double ta, int64_t nb, double tb) {
+    const int64_t full = na / slots, late = na % slots;   // `late` slots take one more of a's
+    const double start = (double)full * ta;
+    int64_t k0 = 0, k1 = 0;   // b's that an early and a late slot take
+    while ((slots - late) * k0 + late * k1 < nb)
+        if (late == 0 || start + (double)(k0 + 1) * tb <= start + ta + (double)(k1 + 1) * tb) ++k0;
+        else ++k1;
+    const double early = start + (double)k0 * tb, last = late ? start + ta + (double)k1 * tb : 0.0;
+    return early > last ? early : last;
+}
+
+// Two products in one launch of one tile, where that is estimated to be faster than a launch each: the
+// second's tiles go where the first's leave room, and about 4 us of a launch's start and end are saved
+// (at 1 % of large ones: dx and dW of 8192 x 4096 x 11264, whose rounds are the same, 2445 us both ways).
+struct Pair {
+    int side;   // 0: a launch each
+    int splits; // of the first product
+};
+Pair plan_pair(const Product& a, const Product& b, int elem) {
+    double ua, ub;
+    plan_product(a, elem, &ua);
+    plan_product(b, elem, &ub);
+    double least = 0.99 * (ua + ub) + 4.0;
+    Pair best{0, 1};
+    for (int side : {256, 128, 64}) {
+        if (!can_take(a, elem, side) || !can_take(b, elem, side)) continue;
+        const int64_t ka = ktiles_of(a, elem), kb = ktiles_of(b, elem), slots = (int64_t)kCus * per_cu(side), nb = tiles_of(b, side);
+        for (int splits = 1; splits <= 32; splits *= 2) {
+            const int64_t na = tiles_of(a, side) * splits;
+            if (splits > 1 && (na > slots || ka / splits < 4)) break;
+            const double full = (double)(na + nb) / slots;
+            const double ta = tile_us(side, elem, (ka + splits - 1) / splits, full), tb = tile_us(side, elem, kb, full);
+            double t = ta > tb ? ta : tb;
+            if (full > 1.0) {   // small tiles have no rounds: a slot is free soon
+                const double run = side == 64 ? ((double)na * ta + (double)nb * tb) / slots : two_runs_us(slots, na, ta, nb, tb);
+                t = run > t ? run : t;
+            }
+            t += join_us(a, splits);
+            if (t < least) least = t, best = Pair{side, splits};
         }
     }
     return best;
 }
-size_t slab_bytes(const Product& p, const Plan& q) {
-    return q.splits > 1 ? (size_t)q.splits * p.a.batch * p.a.M * (size_t)up8(p.a.N) * 4 : 0;
+size_t slab_bytes(const Product& p, int splits) {
+    return splits > 1 ? (size_t)splits * p.a.batch * p.a.M * (size_t)up8(p.a.N) * 4 : 0;
 }
 
 template <typename T, bool TRA, bool TRB, int EPI>
@@ -912,19 +1013,50 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     return hipGetLastError();
 }
 
+// the product with its result in the slabs of `q` where it has some, and what joins them
+GemmArgs slabs(const Product& p, int splits, float* slab) {
+    GemmArgs a = p.a;
+    a.splits = splits;
+    if (splits > 1) a.c[0] = slab, a.ldc = up8(a.N);
+    return a;
+}
+template <typename T> hipError_t join(const Product& p, int splits, const float* slab, hipStream_t s) {
+    if (splits == 1) return hipSuccess;
+    const GemmArgs& a = p.a;
+    const int64_t ldc = up8(a.N), work = (int64_t)a.M * a.batch * (ldc / 4);
+    ffn_join_kernel<T><<<(unsigned)((work + 255) / 256), 256, 0, s>>>(slab, splits, a.batch, a.M, a.N, ldc, (T*)a.c[0],
+                                                                     (T*)a.c[1], a.ldc);
+    return hipGetLastError();
+}
+
 template <typename T, bool TRA, bool TRB>
 hipError_t run_store(const Product& p, float* slab, hipStream_t s) {
     const Plan q = plan_product(p, (int)sizeof(T));
-    if (q.splits == 1) return launch_tiles<T, TRA, TRB, kStore>(p.a, q, s);
-    GemmArgs a = p.a;
-    a.c[0] = slab;
-    a.ldc = up8(a.N);
-    const hipError_t e = launch_tiles<T, TRA, TRB, kPartial>(a, q, s);
-    if (e != hipSuccess) return e;
-    const int64_t work = (int64_t)a.M * a.batch * (a.ldc / 4);
-    ffn_join_kernel<T><<<(unsigned)((work + 255) / 256), 256, 0, s>>>(slab, q.splits, a.batch, a.M, a.N, a.ldc,
-                                                                     (T*)p.a.c[0], (T*)p.a.c[1], p.a.ldc);
-    return hipGetLastError();
+    const hipError_t e = launch_tiles<T, TRA, TRB, kStore>(slabs(p, q.splits, slab), q, s);
+    return e != hipSuccess ? e : join<T>(p, q.splits, slab, s);
+}
+
+template <typename T, bool TRA1, bool TRA2, int EPI2>
+hipError_t run_pair(const Product& p, const Product& second, const Pair& q, float* slab, hipStream_t s) {
+    constexpr int depth = kTileBytes / (int)sizeof(T);
+    GemmArgs a = slabs(p, q.splits, slab), b = second.a;
+    int64_t blocks[2];
+    for (GemmArgs* g : {&a, &b}) {
+        if ((g->a.k + depth - 1) / depth != (g->b.k + depth - 1) / depth) return hipErrorInvalidValue;
+        g->tiles_m = (g->M + q.side - 1) / q.side, g->tiles_n = (g->N + q.side - 1) / q.side;
+        blocks[g == &b] = ((int64_t)g->tiles_m * g->tiles_n + 7) / 8 * 8 * g->batch * g->splits;
+    }
+    const unsigned grid = (unsigned)(blocks[0] + blocks[1]);
+    const int first = (int)blocks[0];
+    if (q.side == 256) {
+        if constexpr (sizeof(T) == 2) ffn_gemm_pair_kernel<T, 256, TRA1, kStore, TRA2, EPI2><<<grid, 512, 0, s>>>(a, b, first);
+    } else if (q.side == 128) {
+        ffn_gemm_pair_kernel<T, 128, TRA1, kStore, TRA2, EPI2><<<grid, 256, 0, s>>>(a, b, first);
+    } else {
+        ffn_gemm_pair_kernel<T, 64, TRA1, kStore, TRA2, EPI2><<<grid, 256, 0, s>>>(a, b, first);
+    }
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : join<T>(p, q.splits, slab, s);
 }
 
 // The block's buffers and products.  Built twice: for the sizes (null pointers) and to run.
@@ -1063,7 +1195,7 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     in.a.b.p[1] = b.wu.p[0];
     in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.fk;
     Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.fk, b.es, b.n, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
-    float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es)));
+    float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es).splits));
     *need = b.ws.used;
     if (!run) return OTF_OK;
     OTF_HIP(b.run_pack<T>(s));
@@ -1126,23 +1258,36 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     pi.a.a.p[1] = du, pi.a.c[1] = o->dw_up, pi.a.batch = 2;
     // dWd = dy^T h
     Product pd{true, true, kStore, product_args(by_columns(b.dy, b.n), buffer_operand(sv.h, b.fk, b.es, b.fk, b.n), b.d, b.f, o->dw_down, o->lddw_down)};
+    // what needs nothing of each other shares a launch: dWd and dh, then dx and dWg, dWu
+    const bool dh = wx || win;
+    const Pair with_dh = dh && wdown && !outer ? plan_pair(pd, mid, b.es) : Pair{0, 1};
+    const Pair with_in = wx && win && !outer ? plan_pair(px, pi, b.es) : Pair{0, 1};
     size_t slab = 0;   // one after another on the stream: they share it
-    auto more = [&](const Product& p) { const size_t k = slab_bytes(p, plan_product(p, b.es)); slab = k > slab ? k : slab; };
-    if (wx) more(px);
-    if (win && !outer) more(pi);
-    if (wdown && !outer) more(pd);
+    auto more = [&](const Product& p, const Pair& q) {
+        const size_t k = slab_bytes(p, q.side ? q.splits : plan_product(p, b.es).splits);
+        slab = k > slab ? k : slab;
+    };
+    if (wx) more(px, with_in);
+    if (win && !outer && !with_in.side) more(pi, Pair{0, 1});
+    if (wdown && !outer) more(pd, with_dh);
     float* part = (float*)b.ws.take(slab);
     *need = b.ws.used;
     if (!run) return OTF_OK;
     OTF_HIP(b.run_pack<T>(s));
-    if (wx || win) OTF_HIP((launch_tiles<T, false, true, kGatedBackward>(mid.a, plan_product(mid, b.es), s)));
-    if (wx) OTF_HIP((run_store<T, false, true>(px, part, s)));
+    if (with_dh.side)
+        OTF_HIP((run_pair<T, true, false, kGatedBackward>(pd, mid, with_dh, part, s)));
+    else if (dh)
+        OTF_HIP((launch_tiles<T, false, true, kGatedBackward>(mid.a, plan_product(mid, b.es), s)));
+    if (with_in.side)
+        OTF_HIP((run_pair<T, false, true, kStore>(px, pi, with_in, part, s)));
+    else if (wx)
+        OTF_HIP((run_store<T, false, true>(px, part, s)));
     if (outer) {
         OTF_HIP((run_outer<T>(b, dg, du, sv.h, s)));
         return OTF_OK;
     }
-    if (win) OTF_HIP((run_store<T, true, true>(pi, part, s)));
-    if (wdown) OTF_HIP((run_store<T, true, true>(pd, part, s)));
+    if (win && !with_in.side) OTF_HIP((run_store<T, true, true>(pi, part, s)));
+    if (wdown && !with_dh.side) OTF_HIP((run_store<T, true, true>(pd, part, s)));
     return OTF_OK;
 }
 

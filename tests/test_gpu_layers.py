@@ -319,6 +319,14 @@ def test_gated_feed_forward(dev, dt, act, rows, d, f):
     assert all(torch.equal(p, q) for p, q in zip(grads, again))
 
 
+# two products a launch with tiles of each side, in slabs and without, tile counts off multiples of eight
+@pytest.mark.parametrize("dt,act,rows,d,f", [("f16", "gelu", 777, 1000, 2730), ("bf16", "silu", 1024, 2048, 2816), ("bf16", "gelu", 3001, 520, 1400),
+                                             ("bf16", "silu", 100, 512, 1408), ("f32", "gelu", 700, 1024, 2050), ("f32", "silu", 260, 500, 2044),
+                                             ("bf16", "silu", 70, 2056, 5000), ("f16", "silu", 2304, 1032, 4104)])
+def test_gated_feed_forward_shared_launches(dev, dt, act, rows, d, f):
+    test_gated_feed_forward(dev, dt, act, rows, d, f)
+
+
 @pytest.mark.parametrize("dt,act,rows,d,f", [("bf16", "gelu", 4200, 4100, 4110), ("f16", "silu", 4097, 4104, 4352)])
 def test_gated_feed_forward_large_tiles(dev, dt, act, rows, d, f):
     """Every product in whole and ragged tiles of the largest size, odd widths among them."""
