@@ -1076,10 +1076,11 @@ struct Block {
         ws.base = (char*)workspace;
     }
 
-    bool aligned(const void* p, int64_t ld, int64_t cols) const {
-        return cols % (whole ? 64 : 8) == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
+    // by_k: the columns are K in some product
+    bool aligned(const void* p, int64_t ld, int64_t cols, bool by_k) const {
+        return cols % (whole && by_k ? 64 : 8) == 0 && ld % 8 == 0 && (uintptr_t)p % 16 == 0;
     }
-    void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols, bool copy) {
+    void place(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols, bool copy) {
         v.p[0] = v.p[1] = (const char*)p;
         v.ld = ld * es;
         v.k = (int)cols;
@@ -1093,14 +1094,14 @@ struct Block {
             v.k = (int)ldd;
         }
     }
-    void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols) {
-        operand(v, p, ld, rows, cols, !aligned(p, ld, cols));
-    }
     // gate and up: one leading dimension, so both are copied or none
-    void weights_in() {
-        const bool copy = !aligned(o->w_gate, o->ldw_in, d) || !aligned(o->w_up, o->ldw_in, d);
-        operand(wg, o->w_gate, o->ldw_in, f, d, copy);
-        operand(wu, o->w_up, o->ldw_in, f, d, copy);
+    void weights_in(bool by_k) {
+        const bool copy = !aligned(o->w_gate, o->ldw_in, d, by_k) || !aligned(o->w_up, o->ldw_in, d, by_k);
+        place(wg, o->w_gate, o->ldw_in, f, d, copy);
+        place(wu, o->w_up, o->ldw_in, f, d, copy);
+    }
+    void operand(Operand& v, const void* p, int64_t ld, int64_t rows, int64_t cols, bool by_k) {
+        place(v, p, ld, rows, cols, !aligned(p, ld, cols, by_k));
     }
     template <typename T> hipError_t run_pack(hipStream_t s) {
         if (!pack.count) return hipSuccess;
@@ -1187,9 +1188,9 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
                                                         nullptr);
         return check_hip(hipGetLastError());
     }
-    b.operand(b.x, o->x, o->ldx, b.n, b.d);
-    b.weights_in();
-    b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
+    b.operand(b.x, o->x, o->ldx, b.n, b.d, true);
+    b.weights_in(true);
+    b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f, true);
     const int kin = b.x.k < b.wg.k ? b.x.k : b.wg.k;   // what is copied ends in zeros
     Product in{false, false, kGatedForward, product_args(by_rows(b.x, b.n, kin), by_rows(b.wg, b.f, kin), b.n, b.fk, nullptr, 0)};
     in.a.b.p[1] = b.wu.p[0];
@@ -1242,11 +1243,11 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
     char* dg = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
     char* du = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
-    b.operand(b.dy, o->dy, o->lddy, b.n, b.d);
-    if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f);
-    if (wx) b.weights_in();
+    b.operand(b.dy, o->dy, o->lddy, b.n, b.d, true);
+    if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f, false);
+    if (wx) b.weights_in(false);
     const bool outer = b.n <= kOuterRows;   // the weights' gradients without tiles
-    if (win && !outer) b.operand(b.x, o->x, o->ldx, b.n, b.d);
+    if (win && !outer) b.operand(b.x, o->x, o->ldx, b.n, b.d, false);
     // dh = dy Wd: K = d, the rows of Wd
     Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.fk, nullptr, 0)};
     mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.fk;
