@@ -198,6 +198,7 @@ struct GemmArgs {
     void* h;             // gated forward: h; backward: dg
     void* h2;            // gated backward: du
     int64_t ldh;         // elements, of g, u, h, h2
+    int low;             // 16-row tiles: A's rows (kStore) or the hidden results' from here on are low parts, 0: none
 };
 
 template <typename T>
@@ -218,6 +219,22 @@ template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
     using V = T __attribute__((ext_vector_type(4)));
     const V q = *reinterpret_cast<const V*>(p);
     return f32x4{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
+}
+
+// A hidden value in 32 bits but for the last: the value's rounding to T, and `low` elements on what
+// that left out (nothing of an overflow).  low = 0: the rounding alone.
+template <typename T> __device__ __forceinline__ void store_hidden(T* p, int64_t low, f32x4 v) {
+    store4(p, 4, true, v);
+    if constexpr (sizeof(T) == 2) {
+        if (low) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float high = (float)(T)v[j];
+                v[j] = fabsf(high) < __builtin_inff() ? v[j] - high : 0.0f;
+            }
+            store4(p + low, 4, true, v);
+        }
+    }
 }
 
 // four consecutive columns n.. of row m: acc0 of the tile's first half, acc1 of its second
@@ -245,7 +262,7 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
             if (n + j >= a.features) acc0[j] = acc1[j] = 0.0f;
             h[j] = act_value<T>(a.act, acc0[j]) * acc1[j];
         }
-        store4((T*)a.h + o, 4, true, h);
+        store_hidden((T*)a.h + o, a.low * a.ldh, h);
         if (a.g) {
             store4(a.g + o, 4, true, acc0);
             store4(a.u + o, 4, true, acc1);
@@ -265,8 +282,8 @@ __device__ __forceinline__ void finish4(const GemmArgs& a, int z, int split, int
                 dg[j] = nn + j < a.features ? dh[j] * u[j] * dv : 0.0f;
                 du[j] = nn + j < a.features ? dh[j] * v : 0.0f;
             }
-            store4((T*)a.h + o, 4, true, dg);
-            store4((T*)a.h2 + o, 4, true, du);
+            store_hidden((T*)a.h + o, a.low * a.ldh, dg);
+            store_hidden((T*)a.h2 + o, a.low * a.ldh, du);
         }
     }
 }
@@ -346,6 +363,14 @@ template <typename T, int R> __device__ __forceinline__ uint32_t tr_address(cons
     const int i = lane & 15, k = (lane >> 4) * 8 + (i >> 2);
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)tile + k * (R * 2) +
            (((r0 / 8 + ((i & 3) >> 1)) ^ swz_t<T, R>(k)) << 4) + (i & 1) * 8;
+}
+
+// a lane's sums of the rows `low` further on in its 16 (those of the low parts)
+__device__ __forceinline__ f32x4 low_rows(f32x4 v, int low) {
+    f32x4 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __shfl(v[j], ((int)threadIdx.x & 48) | (((int)threadIdx.x + low) & 15));
+    return r;
 }
 
 // ---- the tiled product -----------------------------------------------------------------
@@ -471,6 +496,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, int z, int 
             const int m = m0 + (wm * RA + i) * 16 + (lane & 15), n = n0 + (wn * RB + j) * 16 + (lane >> 4) * 4;
             f32x4 r0 = acc[0][0][j][i], r1 = acc[0][1][j][i];
             if constexpr (SUMS == 2) r0 += acc[1][0][j][i], r1 += acc[1][1][j][i];
+            if constexpr (TM == 16 && EPI == kStore && sizeof(T) == 2) {
+                if (a.low) r0 += low_rows(r0, a.low), r1 += low_rows(r1, a.low);
+            }
             finish4<T, EPI>(a, z, split, m, n, n + TH, r0, r1);
         }
 }
@@ -685,12 +713,15 @@ __global__ __launch_bounds__(256) void ffn_join_kernel(const float* __restrict__
 // ---- few rows ------------------------------------------------------------------------------
 // Up to 16 rows of x: the weights are read once, straight into registers, and bound the time.
 // A workgroup takes 16 features (GATED: of both weights); its NW waves take 128-byte pieces of
-// K in turn and meet in LDS.  Rows of x past the last are zero fragments.
+// K in turn and meet in LDS.  Rows of x past the last are zero fragments.  low: GATED, where the
+// low parts of the results go; else the low parts of x follow its rows (low = rows), in MFMA rows
+// that would be zeros.
 template <typename T, bool GATED, int NW>
 __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ x, int64_t ldx, int rows,
                                                           const T* __restrict__ w0, const T* __restrict__ w1,
                                                           int64_t ldw, int K, int N, int act, T* __restrict__ out,
-                                                          int64_t ldo, float* __restrict__ sg, float* __restrict__ su) {
+                                                          int64_t ldo, float* __restrict__ sg, float* __restrict__ su,
+                                                          int low) {
     constexpr int NB = GATED ? 2 : 1, PIECE = 128 / (int)sizeof(T), CH = 16 / (int)sizeof(T);
     constexpr int UNROLL = GATED ? 2 : 4;
     __shared__ f32x4 part[NW][NB][64];
@@ -698,8 +729,8 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
     const int n0 = blockIdx.x * 16;
     const int64_t wrow = n0 + r < N ? n0 + r : N - 1;   // past the end: read the last row, drop the result
     const T* pw[2] = {w0 + wrow * ldw, GATED ? w1 + wrow * ldw : nullptr};
-    const T* px = x + (int64_t)(r < rows ? r : 0) * ldx;
-    const bool live = r < rows;
+    const bool live = r < rows, read = r < rows + (GATED ? 0 : low);
+    const T* px = x + (int64_t)(read ? r : 0) * ldx;
     using F = typename Frag<T>::type;
     using U = T __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
     auto chunk = [&](const T* p, int k) -> F {
@@ -727,7 +758,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
                 const int k = k0 + u * NW * PIECE + (s * 4 + kc) * CH;
 #pragma unroll
                 for (int b = 0; b < NB; ++b) fw[u][s][b] = chunk(pw[b], k);
-                fx[u][s] = live ? chunk(px, k) : F{};
+                fx[u][s] = read ? chunk(px, k) : F{};
             }
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
@@ -747,6 +778,9 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
 #pragma unroll
         for (int w = 1; w < NW; ++w) s[b] += part[w][b][lane];
     }
+    if constexpr (!GATED && sizeof(T) == 2) {
+        if (low) s[0] += low_rows(s[0], low);
+    }
     if (!live) return;
     const int n = n0 + kc * 4;
     if constexpr (GATED) {   // ldo whole K-tiles, columns up to it written (zeros past N)
@@ -758,7 +792,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
         }
         if (n >= ldo) return;
         const int64_t o = (int64_t)r * ldo + n;
-        store4(out + o, 4, true, h);
+        store_hidden(out + o, low * ldo, h);
         if (sg) {
             store4(sg + o, 4, true, s[0]);
             store4(su + o, 4, true, s[1]);
@@ -778,6 +812,7 @@ struct OuterJob {
     const void *a, *b;
     void* c;
     int64_t lda, ldb, ldc;
+    int64_t low_a, low_b;   // elements to the low parts, 0: none
     int R, C;
     int across;     // threads across the columns, a power of two from 32 to 256
     int wide;       // workgroups across the columns
@@ -797,7 +832,13 @@ template <typename T, int NR> __global__ __launch_bounds__(256) void ffn_outer_k
     const int r0 = (block / j.wide) * RB, col = ((block % j.wide) * j.across + tx) * 8;
     for (int i = threadIdx.x; i < NR * RB; i += 256) {
         const int n = i / RB, r = r0 + i % RB;
-        sa[i] = n < o.rows && r < j.R ? (float)((const T*)j.a)[n * j.lda + r] : 0.0f;
+        float a = 0.0f;
+        if (n < o.rows && r < j.R) {
+            const T* p = (const T*)j.a + n * j.lda + r;
+            a = (float)p[0];
+            if (j.low_a) a += (float)p[j.low_a];
+        }
+        sa[i] = a;
     }
     __syncthreads();
     const int valid = j.C - col;
@@ -806,7 +847,14 @@ template <typename T, int NR> __global__ __launch_bounds__(256) void ffn_outer_k
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
         if (n < o.rows) {
-            load8((const T*)j.b + n * j.ldb + col, valid, b[n]);
+            const T* p = (const T*)j.b + n * j.ldb + col;
+            load8(p, valid, b[n]);
+            if (j.low_b) {
+                float l[8];
+                load8(p + j.low_b, valid, l);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) b[n][q] += l[q];
+            }
         } else {
 #pragma unroll
             for (int q = 0; q < 8; ++q) b[n][q] = 0.0f;
@@ -905,6 +953,7 @@ int64_t ktiles_of(const Product& p, int elem) {
 }
 bool can_take(const Product& p, int elem, int side) {
     if (side == 16) return !p.tra && p.a.M <= 16;
+    if (p.a.low) return false;
     return side != 256 || (elem == 2 && (p.tra || p.a.a.k % 64 == 0) && (p.trb || p.a.b.k % 64 == 0));
 }
 // a tile of this many K-tiles where the launch fills `full` of the chip's slots
@@ -1059,11 +1108,17 @@ hipError_t run_pair(const Product& p, const Product& second, const Pair& q, floa
     return e != hipSuccess ? e : join<T>(p, q.splits, slab, s);
 }
 
+// Up to 8 rows of 16-bit operands: the hidden values (h, dg, du) keep their low parts, as many more
+// rows that a 16-row tile has room for, so that only the results are rounded (y of one token 1.0
+// instead of 1.4 times its rounding off).  More rows would cost MFMAs and passes over the hidden values.
+int low_rows_of(int64_t rows, int es) { return es == 2 && rows <= 8 ? (int)rows : 0; }
 // The block's buffers and products.  Built twice: for the sizes (null pointers) and to run.
 struct Block {
     const otf_ffn_args* o;
     int es;
     int64_t n, d, f, fk;    // fk: f in whole K-tiles, the hidden buffers' leading dimension, zeros past f
+    int low;                // rows of low parts after a hidden buffer's
+    int64_t nh;             // its rows with them
     bool whole;             // operands copied to whole K-tiles (large products of ragged widths)
     Operand x{}, wg{}, wu{}, wd{}, dy{};   // k: columns there are, zeros past the caller's
     PackArgs pack{};
@@ -1071,6 +1126,7 @@ struct Block {
 
     Block(const otf_ffn_args* args, int elem, void* workspace) : o(args), es(elem) {
         n = o->rows, d = o->d, f = o->f, fk = up_ktile(f, es);
+        low = low_rows_of(n, es), nh = n + low;
         // ragged widths: a copy costs two passes over the operands, and pays where the products are large
         whole = es == 2 && ((n + 255) / 256) * ((f + 127) / 128) >= kCus;
         ws.base = (char*)workspace;
@@ -1165,7 +1221,9 @@ Saved carve_saved(void* p, int64_t n, int64_t fk, int es) {
     const size_t wide = up256((size_t)(n * fk) * 4);
     return Saved{(float*)b, (float*)(b + wide), b + 2 * wide};
 }
-size_t saved_bytes(int64_t n, int64_t fk, int es) { return 2 * up256((size_t)(n * fk) * 4) + up256((size_t)(n * fk * es)); }
+size_t saved_bytes(int64_t n, int64_t fk, int es) {
+    return 2 * up256((size_t)(n * fk) * 4) + up256((size_t)((n + low_rows_of(n, es)) * fk * es));
+}
 
 // forward: the workspace it needs in *need; runs where run is set
 template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
@@ -1174,18 +1232,18 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     if (o->saved)
         sv = carve_saved(o->saved, b.n, b.fk, b.es);
     else
-        sv.h = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
+        sv.h = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
     if (few_rows(b.n, b.d, b.f, b.es)) {
         *need = b.ws.used;
         if (!run) return OTF_OK;
         const unsigned g1 = (unsigned)((b.fk + 15) / 16), g2 = (unsigned)((b.d + 15) / 16);
         ffn_few_kernel<T, true, 4><<<g1, 256, 0, s>>>((const T*)o->x, o->ldx, (int)b.n, (const T*)o->w_gate,
                                                        (const T*)o->w_up, o->ldw_in, (int)b.d, (int)b.f, o->activation,
-                                                       (T*)sv.h, b.fk, sv.g, sv.u);
+                                                       (T*)sv.h, b.fk, sv.g, sv.u, b.low);
         OTF_HIP(hipGetLastError());
         ffn_few_kernel<T, false, 8><<<g2, 512, 0, s>>>((const T*)sv.h, b.fk, (int)b.n, (const T*)o->w_down, nullptr,
                                                         o->ldw_down, (int)b.f, (int)b.d, 0, (T*)o->y, o->ldy, nullptr,
-                                                        nullptr);
+                                                        nullptr, b.low);
         return check_hip(hipGetLastError());
     }
     b.operand(b.x, o->x, o->ldx, b.n, b.d, true);
@@ -1194,8 +1252,9 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     const int kin = b.x.k < b.wg.k ? b.x.k : b.wg.k;   // what is copied ends in zeros
     Product in{false, false, kGatedForward, product_args(by_rows(b.x, b.n, kin), by_rows(b.wg, b.f, kin), b.n, b.fk, nullptr, 0)};
     in.a.b.p[1] = b.wu.p[0];
-    in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.fk;
-    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.fk, b.es, b.n, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
+    in.a.act = o->activation, in.a.features = (int)b.f, in.a.g = sv.g, in.a.u = sv.u, in.a.h = sv.h, in.a.ldh = b.fk, in.a.low = b.low;
+    Product down{false, false, kStore, product_args(buffer_operand(sv.h, b.fk, b.es, b.nh, b.wd.k), by_rows(b.wd, b.d, b.wd.k), b.n, b.d, o->y, o->ldy)};
+    down.a.low = b.low;
     float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es).splits));
     *need = b.ws.used;
     if (!run) return OTF_OK;
@@ -1215,18 +1274,18 @@ hipError_t run_outer(const Block& b, const char* dg, const char* du, const char*
     args.rows = (int)b.n;
     args.walk = b.d * b.f >= (int64_t)1 << 23 ? 16 : 4;   // 2^23: about 1024 workgroups of 16 rows by 256 threads
     int64_t blocks = 0;
-    auto add = [&](const void* a, int64_t lda, int64_t R, const void* bb, int64_t ldb, int64_t C, void* c, int64_t ldc) {
+    auto add = [&](const void* a, int64_t lda, int64_t low_a, int64_t R, const void* bb, int64_t ldb, int64_t low_b, int64_t C, void* c, int64_t ldc) {
         int across = 32;
         while (across < 256 && across * 8 < C) across *= 2;
         const int64_t wide = (C + across * 8 - 1) / (across * 8), deep = args.walk * (256 / across);
-        args.job[args.count++] = OuterJob{a, bb, c, lda, ldb, ldc, (int)R, (int)C, across, (int)wide, blocks};
+        args.job[args.count++] = OuterJob{a, bb, c, lda, ldb, ldc, low_a, low_b, (int)R, (int)C, across, (int)wide, blocks};
         blocks += wide * ((R + deep - 1) / deep);
     };
     if (o->dw_gate) {
-        add(dg, b.fk, b.f, o->x, o->ldx, b.d, o->dw_gate, o->lddw_in);
-        add(du, b.fk, b.f, o->x, o->ldx, b.d, o->dw_up, o->lddw_in);
+        add(dg, b.fk, b.low * b.fk, b.f, o->x, o->ldx, 0, b.d, o->dw_gate, o->lddw_in);
+        add(du, b.fk, b.low * b.fk, b.f, o->x, o->ldx, 0, b.d, o->dw_up, o->lddw_in);
     }
-    if (o->dw_down) add(o->dy, o->lddy, b.d, h, b.fk, b.f, o->dw_down, o->lddw_down);
+    if (o->dw_down) add(o->dy, o->lddy, 0, b.d, h, b.fk, b.low * b.fk, b.f, o->dw_down, o->lddw_down);
     if (!args.count) return hipSuccess;
     if (b.n <= 4)
         ffn_outer_kernel<T, 4><<<(unsigned)blocks, 256, 0, s>>>(args);
@@ -1241,8 +1300,8 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     Block b(o, (int)sizeof(T), workspace);
     const Saved sv = carve_saved(o->saved, b.n, b.fk, b.es);
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
-    char* dg = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
-    char* du = (char*)b.ws.take((size_t)(b.n * b.fk * b.es));
+    char* dg = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
+    char* du = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
     b.operand(b.dy, o->dy, o->lddy, b.n, b.d, true);
     if (wx || win) b.operand(b.wd, o->w_down, o->ldw_down, b.d, b.f, false);
     if (wx) b.weights_in(false);
@@ -1250,10 +1309,10 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     if (win && !outer) b.operand(b.x, o->x, o->ldx, b.n, b.d, false);
     // dh = dy Wd: K = d, the rows of Wd
     Product mid{false, true, kGatedBackward, product_args(by_rows(b.dy, b.n, b.dy.k), by_columns(b.wd, b.d), b.n, b.fk, nullptr, 0)};
-    mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.fk;
+    mid.a.act = o->activation, mid.a.features = (int)b.f, mid.a.g = sv.g, mid.a.u = sv.u, mid.a.h = dg, mid.a.h2 = du, mid.a.ldh = b.fk, mid.a.low = b.low;
     // dx = dg Wg + du Wu: two segments of K = f, the rows of the weights
-    Product px{false, true, kStore, product_args(buffer_operand(dg, b.fk, b.es, b.n, b.fk), by_columns(b.wg, b.f), b.n, b.d, o->dx, o->lddx)};
-    px.a.a.p[1] = du, px.a.b.p[1] = b.wu.p[0], px.a.segments = 2;
+    Product px{false, true, kStore, product_args(buffer_operand(dg, b.fk, b.es, b.nh, b.fk), by_columns(b.wg, b.f), b.n, b.d, o->dx, o->lddx)};
+    px.a.a.p[1] = du, px.a.b.p[1] = b.wu.p[0], px.a.segments = 2, px.a.low = b.low;
     // dWg, dWu = dg^T x, du^T x: a batch of two, K = rows
     Product pi{true, true, kStore, product_args(buffer_operand(dg, b.fk, b.es, b.fk, b.n), by_columns(b.x, b.n), b.f, b.d, o->dw_gate, o->lddw_in)};
     pi.a.a.p[1] = du, pi.a.c[1] = o->dw_up, pi.a.batch = 2;

@@ -327,6 +327,38 @@ def test_gated_feed_forward_shared_launches(dev, dt, act, rows, d, f):
     test_gated_feed_forward(dev, dt, act, rows, d, f)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,d,f", [(1, 256, 96), (2, 128, 302), (5, 72, 1100), (8, 1024, 2050), (8, 2048, 4104), (3, 4096, 5632)])
+def test_gated_feed_forward_few_rows_round_once(dev, dt, rows, d, f):
+    """Up to eight rows: what lies between x and a result is held in 32 bits, or in 16 with what they
+    leave out, 2^-16 and better of a value.  So a result differs from the rounding of the 64-bit one
+    only where that lies within the sums' error of a tie: 2^-16 of the sum's terms, against a step of
+    2^-7 or 2^-10 of the value, 2^-5 of the results at most for values of the terms' size (a hidden
+    value rounded to T, half a step off itself, would move about a third of them)."""
+    from otfuse import layers
+    t = T[dt]
+    x = _randn(dev, 1, rows, d, dtype=t)
+    w = [_randn(dev, i, *s, dtype=t, scale=s[1] ** -0.5) for i, s in ((2, (f, d)), (3, (f, d)), (4, (d, f)))]
+    dy = _randn(dev, 5, rows, d, dtype=t)
+    args = [v.requires_grad_(True) for v in (x, *w)]
+    y = layers.gated_feed_forward(*args)
+    got = (y, *torch.autograd.grad(y, args, dy))
+    ref = plain.gated_feed_forward(*(v.detach().double() for v in args), "silu", dy.double())
+    for g, r in zip(got, ref):
+        assert (g.detach() != r.to(t)).double().mean() <= 2.0 ** -4
+
+
+def test_gated_feed_forward_few_rows_overflow(dev):
+    """A hidden value past float16 is an infinity, as one rounding makes it, not a NaN."""
+    from otfuse import layers
+    x = torch.full((2, 64), 64.0, dtype=torch.float16, device=dev)
+    x[1] = 0.25
+    w = torch.full((16, 64), 0.25, dtype=torch.float16, device=dev)
+    down = torch.full((64, 16), 0.5, dtype=torch.float16, device=dev)
+    y = layers.gated_feed_forward(x, w, w, down)   # gate and up 1024: 2^20 hidden
+    assert torch.isinf(y[0]).all() and torch.isfinite(y[1]).all()
+
+
 @pytest.mark.parametrize("dt,act,rows,d,f", [("bf16", "gelu", 4200, 4100, 4110), ("f16", "silu", 4097, 4104, 4352)])
 def test_gated_feed_forward_large_tiles(dev, dt, act, rows, d, f):
     """Every product in whole and ragged tiles of the largest size, odd widths among them."""
