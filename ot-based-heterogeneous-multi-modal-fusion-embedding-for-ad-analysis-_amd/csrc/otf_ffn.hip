@@ -13,7 +13,7 @@
 // is transposed on the way from LDS to registers (ds_read_b64_tr_b16).
 //
 // All sums are float32 in the accumulators.  h, dg and du are rounded to the operands' type, which
-// the products that read them need; g and u are kept in float32 for the backward pass, where their
+// the products that read them need (up to 8 rows with their low parts beside them); g and u are kept in float32 for the backward pass, where their
 // rounding would meet dg's and du's own (gradients of 16-bit operands then err by 1.4 times their
 // final rounding instead of 1.8; at 8192 x 4096 x 11264 the wider buffers cost 2 % of a step).
 #include "otf_rng.h"
@@ -805,7 +805,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
 
 // ---- weight gradients of few rows -------------------------------------------------------------
 // C[r, c] = sum_n A[n, r] B[n, c] over up to NR rows, up to three such sums in one launch: bound by
-// the writing of C (bf16, 4096 x 11264, 1 to 8 rows: the three take 60 us where tiles take 120).  A
+// the writing of C (bf16, 4096 x 11264, 1 row: the three take 45 us where tiles take 120).  A
 // thread holds its 8 columns of B's rows in registers and walks `walk` rows of C, 16 or, where that
 // leaves CUs idle, 4; A's values come from LDS.
 struct OuterJob {
@@ -873,6 +873,68 @@ template <typename T, int NR> __global__ __launch_bounds__(256) void ffn_outer_k
             for (int q = 0; q < 8; ++q) v[q] += a * b[n][q];
         }
         store8((T*)j.c + (int64_t)r * j.ldc + col, valid, v);
+    }
+}
+
+// The same sums of 5 to 16 rows of 16-bit operands by MFMA, one step of 16 terms (with the low
+// parts: up to 8 rows and as many more), so that they too are bound by the writing: bf16, 4096 x 11264,
+// 8 rows 65 -> 56 us, 16 rows 102 -> 56; 1 row, without the MFMA, 45 instead of 59.
+// A wave takes 128 columns (64: 59 us) and walks `walk` blocks of 16 rows of C.  A fragment's row i
+// of column block x stands for column (x / 2) 32 + (i / 4) 8 + (x % 2) 4 + i % 4, so that a lane ends with
+// runs of 8 columns of a row, four lanes' beside each other.
+template <typename T> struct Outer;
+template <> struct Outer<_Float16> {
+    typedef __attribute__((ext_vector_type(4))) _Float16 type;
+    static __device__ __forceinline__ f32x4 mma(type a, type b) {
+        return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    }
+};
+template <> struct Outer<__bf16> {
+    typedef __attribute__((ext_vector_type(4))) __bf16 type;
+    static __device__ __forceinline__ f32x4 mma(type a, type b) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b),
+                                                         f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+    }
+};
+template <typename T> __global__ __launch_bounds__(256) void ffn_outer_mfma_kernel(OuterArgs o) {
+    int k = 0;
+    while (k + 1 < o.count && blockIdx.x >= o.job[k + 1].first) ++k;
+    const OuterJob& j = o.job[k];
+    const int block = (int)(blockIdx.x - j.first), lane = threadIdx.x & 63, q = lane >> 4, i = lane & 15;
+    const int r0 = (block / j.wide) * o.walk * 16, c0 = (block % j.wide) * 512 + (threadIdx.x >> 6) * 128;
+    if (c0 >= j.C) return;
+    const int terms = j.low_a || j.low_b ? 2 * o.rows : o.rows;
+    // this lane's four terms of operand p at column `at` of `width`; a term past the rows: the low part
+    auto four = [&](const T* p, int64_t ld, int64_t low, int at, int width) {
+        typename Outer<T>::type v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int n = q * 4 + e;
+            const bool second = n >= o.rows;
+            v[e] = n < terms && at < width ? p[(second ? n - o.rows : n) * ld + (second ? low : 0) + at] : (T)0.0f;
+        }
+        return v;
+    };
+    typename Outer<T>::type b[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) b[x] = four((const T*)j.b, j.ldb, j.low_b, c0 + (x >> 1) * 32 + (i >> 2) * 8 + (x & 1) * 4 + (i & 3), j.C);
+    const int col = c0 + q * 8, last = min(j.R, r0 + o.walk * 16);
+    typename Outer<T>::type a = four((const T*)j.a, j.lda, j.low_a, r0 + i, j.R);
+    for (int r = r0; r < last; r += 16) {
+        const typename Outer<T>::type now = a;
+        a = four((const T*)j.a, j.lda, j.low_a, r + 16 + i, last);
+        float v[4][8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const f32x4 s = Outer<T>::mma(b[x], now);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[x >> 1][(x & 1) * 4 + e] = s[e];
+        }
+        if (r + i >= last) continue;
+        T* c = (T*)j.c + (int64_t)(r + i) * j.ldc + col;
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+            if (j.C - col > h * 32) store8(c + h * 32, j.C - col - h * 32, v[h]);
     }
 }
 
@@ -1110,7 +1172,8 @@ hipError_t run_pair(const Product& p, const Product& second, const Pair& q, floa
 
 // Up to 8 rows of 16-bit operands: the hidden values (h, dg, du) keep their low parts, as many more
 // rows that a 16-row tile has room for, so that only the results are rounded (y of one token 1.0
-// instead of 1.4 times its rounding off).  More rows would cost MFMAs and passes over the hidden values.
+// instead of 1.4 times its rounding off).  More rows would cost MFMAs and passes over the hidden
+// values.  A weight or gradient that is infinite meets both parts, and can give NaN for infinity.
 int low_rows_of(int64_t rows, int es) { return es == 2 && rows <= 8 ? (int)rows : 0; }
 // The block's buffers and products.  Built twice: for the sizes (null pointers) and to run.
 struct Block {
@@ -1272,12 +1335,15 @@ hipError_t run_outer(const Block& b, const char* dg, const char* du, const char*
     const otf_ffn_args* o = b.o;
     OuterArgs args{};
     args.rows = (int)b.n;
-    args.walk = b.d * b.f >= (int64_t)1 << 23 ? 16 : 4;   // 2^23: about 1024 workgroups of 16 rows by 256 threads
+    const bool mfma = sizeof(T) == 2 && b.n > 4;
+    // a thousand workgroups of 16 rows by 256 threads, or by MFMA of 128 rows by 512 columns: else shorter walks
+    args.walk = mfma ? (b.d * b.f >= (int64_t)1 << 24 ? 8 : 4) : b.d * b.f >= (int64_t)1 << 23 ? 16 : 4;
     int64_t blocks = 0;
     auto add = [&](const void* a, int64_t lda, int64_t low_a, int64_t R, const void* bb, int64_t ldb, int64_t low_b, int64_t C, void* c, int64_t ldc) {
         int across = 32;
         while (across < 256 && across * 8 < C) across *= 2;
-        const int64_t wide = (C + across * 8 - 1) / (across * 8), deep = args.walk * (256 / across);
+        const int64_t wide = mfma ? (C + 511) / 512 : (C + across * 8 - 1) / (across * 8);
+        const int64_t deep = args.walk * (mfma ? 16 : 256 / across);
         args.job[args.count++] = OuterJob{a, bb, c, lda, ldb, ldc, low_a, low_b, (int)R, (int)C, across, (int)wide, blocks};
         blocks += wide * ((R + deep - 1) / deep);
     };
@@ -1287,12 +1353,19 @@ hipError_t run_outer(const Block& b, const char* dg, const char* du, const char*
     }
     if (o->dw_down) add(o->dy, o->lddy, 0, b.d, h, b.fk, b.low * b.fk, b.f, o->dw_down, o->lddw_down);
     if (!args.count) return hipSuccess;
-    if (b.n <= 4)
-        ffn_outer_kernel<T, 4><<<(unsigned)blocks, 256, 0, s>>>(args);
-    else if (b.n <= 8)
-        ffn_outer_kernel<T, 8><<<(unsigned)blocks, 256, 0, s>>>(args);
-    else
-        ffn_outer_kernel<T, kOuterRows><<<(unsigned)blocks, 256, 0, s>>>(args);
+    if constexpr (sizeof(T) == 2) {
+        if (mfma)
+            ffn_outer_mfma_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(args);
+        else
+            ffn_outer_kernel<T, 4><<<(unsigned)blocks, 256, 0, s>>>(args);
+    } else {
+        if (b.n <= 4)
+            ffn_outer_kernel<T, 4><<<(unsigned)blocks, 256, 0, s>>>(args);
+        else if (b.n <= 8)
+            ffn_outer_kernel<T, 8><<<(unsigned)blocks, 256, 0, s>>>(args);
+        else
+            ffn_outer_kernel<T, kOuterRows><<<(unsigned)blocks, 256, 0, s>>>(args);
+    }
     return hipGetLastError();
 }
 
