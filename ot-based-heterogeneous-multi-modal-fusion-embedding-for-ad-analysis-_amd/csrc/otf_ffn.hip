@@ -1288,8 +1288,8 @@ size_t saved_bytes(int64_t n, int64_t fk, int es) {
     return 2 * up256((size_t)(n * fk) * 4) + up256((size_t)((n + low_rows_of(n, es)) * fk * es));
 }
 
-// forward: the workspace it needs in *need; runs where run is set
-template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
+// forward: the workspace it needs in *need; runs where `have` is given, the bytes that there are
+template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t* need, const size_t* have, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
     Saved sv{};
     if (o->saved)
@@ -1298,7 +1298,8 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
         sv.h = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
     if (few_rows(b.n, b.d, b.f, b.es)) {
         *need = b.ws.used;
-        if (!run) return OTF_OK;
+        if (!have) return OTF_OK;
+        if (*need && (!workspace || *have < *need)) return OTF_EINVAL;
         const unsigned g1 = (unsigned)((b.fk + 15) / 16), g2 = (unsigned)((b.d + 15) / 16);
         ffn_few_kernel<T, true, 4><<<g1, 256, 0, s>>>((const T*)o->x, o->ldx, (int)b.n, (const T*)o->w_gate,
                                                        (const T*)o->w_up, o->ldw_in, (int)b.d, (int)b.f, o->activation,
@@ -1320,7 +1321,8 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     down.a.low = b.low;
     float* slab = (float*)b.ws.take(slab_bytes(down, plan_product(down, b.es).splits));
     *need = b.ws.used;
-    if (!run) return OTF_OK;
+    if (!have) return OTF_OK;
+    if (*need && (!workspace || *have < *need)) return OTF_EINVAL;
     OTF_HIP(b.run_pack<T>(s));
     OTF_HIP((launch_tiles<T, false, false, kGatedForward>(in.a, plan_product(in, b.es), s)));
     OTF_HIP((run_store<T, false, false>(down, slab, s)));
@@ -1369,7 +1371,7 @@ hipError_t run_outer(const Block& b, const char* dg, const char* du, const char*
     return hipGetLastError();
 }
 
-template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, bool run, hipStream_t s) {
+template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, const size_t* have, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
     const Saved sv = carve_saved(o->saved, b.n, b.fk, b.es);
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
@@ -1405,7 +1407,8 @@ template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_
     if (wdown && !outer) more(pd, with_dh);
     float* part = (float*)b.ws.take(slab);
     *need = b.ws.used;
-    if (!run) return OTF_OK;
+    if (!have) return OTF_OK;
+    if (*need && (!workspace || *have < *need)) return OTF_EINVAL;
     OTF_HIP(b.run_pack<T>(s));
     if (with_dh.side)
         OTF_HIP((run_pair<T, true, false, kGatedBackward>(pd, mid, with_dh, part, s)));
@@ -1430,15 +1433,15 @@ template <typename T> hipError_t zero_rows(void* p, int64_t rows, int64_t cols, 
     return hipGetLastError();
 }
 
-int forward_any(const otf_ffn_args* o, void* ws, size_t* need, bool run, hipStream_t s) {
-    if (o->dtype == OTF_F32) return forward<float>(o, ws, need, run, s);
-    if (o->dtype == OTF_F16) return forward<_Float16>(o, ws, need, run, s);
-    return forward<__bf16>(o, ws, need, run, s);
+int forward_any(const otf_ffn_args* o, void* ws, size_t* need, const size_t* have, hipStream_t s) {
+    if (o->dtype == OTF_F32) return forward<float>(o, ws, need, have, s);
+    if (o->dtype == OTF_F16) return forward<_Float16>(o, ws, need, have, s);
+    return forward<__bf16>(o, ws, need, have, s);
 }
-int backward_any(const otf_ffn_args* o, void* ws, size_t* need, bool run, hipStream_t s) {
-    if (o->dtype == OTF_F32) return backward<float>(o, ws, need, run, s);
-    if (o->dtype == OTF_F16) return backward<_Float16>(o, ws, need, run, s);
-    return backward<__bf16>(o, ws, need, run, s);
+int backward_any(const otf_ffn_args* o, void* ws, size_t* need, const size_t* have, hipStream_t s) {
+    if (o->dtype == OTF_F32) return backward<float>(o, ws, need, have, s);
+    if (o->dtype == OTF_F16) return backward<_Float16>(o, ws, need, have, s);
+    return backward<__bf16>(o, ws, need, have, s);
 }
 
 }  // namespace
@@ -1456,14 +1459,14 @@ size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype) {
 size_t otf_gated_ffn_workspace_size(const otf_ffn_args* o) {
     size_t need = 0;
     if (check_ffn(o) != OTF_OK || o->rows == 0) return 0;
-    forward_any(o, nullptr, &need, false, nullptr);
+    forward_any(o, nullptr, &need, nullptr, nullptr);
     return need;
 }
 
 size_t otf_gated_ffn_backward_workspace_size(const otf_ffn_args* o) {
     size_t need = 0;
     if (check_ffn(o) != OTF_OK || o->rows == 0) return 0;
-    backward_any(o, nullptr, &need, false, nullptr);
+    backward_any(o, nullptr, &need, nullptr, nullptr);
     return need;
 }
 
@@ -1476,10 +1479,7 @@ int otf_gated_ffn(const otf_ffn_args* o, void* workspace, size_t workspace_bytes
         if (misaligned(p, o->dtype)) return OTF_EINVAL;
     if ((uintptr_t)o->saved % 16 || (uintptr_t)workspace % 16) return OTF_EINVAL;
     size_t need = 0;
-    const int rs = forward_any(o, nullptr, &need, false, nullptr);
-    if (rs != OTF_OK) return rs;
-    if (need && (!workspace || workspace_bytes < need)) return OTF_EINVAL;
-    return forward_any(o, workspace, &need, true, (hipStream_t)stream);
+    return forward_any(o, workspace, &need, &workspace_bytes, (hipStream_t)stream);
 }
 
 int otf_gated_ffn_backward(const otf_ffn_args* o, void* workspace, size_t workspace_bytes, otf_stream_t stream) {
@@ -1506,10 +1506,7 @@ int otf_gated_ffn_backward(const otf_ffn_args* o, void* workspace, size_t worksp
         if (misaligned(p, o->dtype)) return OTF_EINVAL;
     if ((uintptr_t)o->saved % 16 || (uintptr_t)workspace % 16) return OTF_EINVAL;
     size_t need = 0;
-    const int rs = backward_any(o, nullptr, &need, false, nullptr);
-    if (rs != OTF_OK) return rs;
-    if (need && (!workspace || workspace_bytes < need)) return OTF_EINVAL;
-    return backward_any(o, workspace, &need, true, s);
+    return backward_any(o, workspace, &need, &workspace_bytes, s);
 }
 
 }  // extern "C"
