@@ -198,7 +198,8 @@ struct GemmArgs {
     void* h;             // gated forward: h; backward: dg
     void* h2;            // gated backward: du
     int64_t ldh;         // elements, of g, u, h, h2
-    int low;             // 16-row tiles: A's rows (kStore) or the hidden results' from here on are low parts, 0: none
+    int low;             // 16-row tiles: A's rows (kStore) or the hidden results' from here on are
+                         // low parts; 0: none
 };
 
 template <typename T>
@@ -994,8 +995,9 @@ constexpr int kCus = 256;   // MI355X; only tile choice depends on it
 
 // Tile side and slabs of K, by the least estimated time.  A CU holds one tile of 256, two of 128,
 // three of 64 or five of 16 by 64; a K-tile then takes it c microseconds (less where it holds
-// fewer), a tile's start and results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted to bf16 products of 64 to
-// 4096 rows by 512 to 4096 and 1408 to 11264 columns, each run with all three sides:
+// fewer), a tile's start and results e, and slabs are written at 4 and joined at 6.4 TB/s.  Fitted
+// to bf16 products of 64 to 4096 rows by 512 to 4096 and 1408 to 11264 columns, each run with all
+// three sides:
 //   gate and up 1024 x 2048 x 5632   62 / 91 / 85 us with 256 / 128 / 64   (176, 704, 2816 tiles)
 //               64 x 4096 x 11264    85 / 93 / 58                          (88, 176, 352)
 //   dh          1024 x 2048 x 5632   78 / 50 / 60                          (88, 352, 1408)
@@ -1105,7 +1107,10 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
     a.tiles_n = (a.N + cols - 1) / cols;
     const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), (unsigned)(a.batch * q.splits));
     if (q.side == 256) {
-        if constexpr (sizeof(T) == 2) ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
+        if constexpr (sizeof(T) == 2)
+            ffn_gemm256_kernel<T, TRA, TRB, EPI><<<grid, 512, 0, s>>>(a);
+        else
+            return hipErrorInvalidValue;
     } else if (q.side == 128) {
         // a third buffer where a CU has only one tile: 4096 x 1024 x 4096, down product, 82 -> 56 us.  With
         // a T operand it gains nothing, and two tiles of two buffers are faster where there are more.
@@ -1117,7 +1122,10 @@ hipError_t launch_tiles(GemmArgs a, const Plan& q, hipStream_t s) {
         }
         ffn_gemm_kernel<T, TRA, TRB, 128, 128, 2, 2, 2, EPI><<<grid, 256, 0, s>>>(a);
     } else if (q.side == 16) {   // up to 16 rows: a taller tile's MFMAs would be spent on rows that are not there
-        if constexpr (!TRA) ffn_gemm_kernel<T, TRA, TRB, 16, 64, 1, 2, 3, EPI><<<grid, 128, 0, s>>>(a);
+        if constexpr (!TRA && (TRB || sizeof(T) == 2))   // float32's forward takes the few-rows kernel
+            ffn_gemm_kernel<T, TRA, TRB, 16, 64, 1, 2, 3, EPI><<<grid, 128, 0, s>>>(a);
+        else
+            return hipErrorInvalidValue;
     } else {
         ffn_gemm_kernel<T, TRA, TRB, 64, 64, 2, 2, 3, EPI><<<grid, 256, 0, s>>>(a);
     }
@@ -1160,7 +1168,10 @@ hipError_t run_pair(const Product& p, const Product& second, const Pair& q, floa
     const unsigned grid = (unsigned)(blocks[0] + blocks[1]);
     const int first = (int)blocks[0];
     if (q.side == 256) {
-        if constexpr (sizeof(T) == 2) ffn_gemm_pair_kernel<T, 256, TRA1, kStore, TRA2, EPI2><<<grid, 512, 0, s>>>(a, b, first);
+        if constexpr (sizeof(T) == 2)
+            ffn_gemm_pair_kernel<T, 256, TRA1, kStore, TRA2, EPI2><<<grid, 512, 0, s>>>(a, b, first);
+        else
+            return hipErrorInvalidValue;
     } else if (q.side == 128) {
         ffn_gemm_pair_kernel<T, 128, TRA1, kStore, TRA2, EPI2><<<grid, 256, 0, s>>>(a, b, first);
     } else {
