@@ -11,8 +11,10 @@ MRI_PET_OT_OT_per_epoch_attn.py:963-1065).  Here:
     gated_feed_forward       (act(x Wg^T) * (x Wu^T)) Wd^T on the matrix cores
 
 Tensors live on a ROCm device; kernels run on the current stream of the tensors' device and
-nothing synchronises, so every call can be captured into a graph.  Inputs are float32,
-bfloat16 or float16; statistics and sums are float32.  Each function takes part in autograd;
+nothing synchronises, so every call can be captured into a graph: forward and backward together,
+and with no eager graph of the same leaves alive (autograd runs a node on the stream that its
+forward, or a leaf's first use in a graph that lives, ran on).  Inputs are float32, bfloat16 or
+float16; statistics and sums are float32.  Each function takes part in autograd;
 without a gradient to compute, nothing is kept for backward.
 """
 from __future__ import annotations
