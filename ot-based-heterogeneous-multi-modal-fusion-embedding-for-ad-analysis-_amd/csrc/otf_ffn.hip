@@ -645,6 +645,9 @@ __device__ __forceinline__ void gemm256_tile(const GemmArgs& a, int id, int z, i
     if (group == 1) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     read_b(0, I0{});
+    // group 1 reads here what group 0 restages after one more barrier, a phase sooner than in later
+    // K-tiles: its reads have returned before that barrier
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     for (int kt = k0; kt < k1; kt += 2) {
         k_tile(kt, I0{});
         if (kt + 1 < k1) k_tile(kt + 1, I1{});
