@@ -955,7 +955,7 @@ struct PackArgs {
     int64_t total;
 };
 template <typename T> __global__ __launch_bounds__(256) void ffn_pack_kernel(PackArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t i = block_id() * 256 + threadIdx.x;
     if (i >= a.total) return;
     int k = 0;
     while (k + 1 < a.count && i >= a.item[k + 1].first) ++k;
@@ -1238,7 +1238,7 @@ struct Block {
     }
     template <typename T> hipError_t run_pack(hipStream_t s) {
         if (!pack.count) return hipSuccess;
-        ffn_pack_kernel<T><<<(unsigned)((pack.total + 255) / 256), 256, 0, s>>>(pack);
+        ffn_pack_kernel<T><<<blocks((pack.total + 255) / 256), 256, 0, s>>>(pack);
         return hipGetLastError();
     }
 };
@@ -1280,7 +1280,7 @@ int check_ffn(const otf_ffn_args* o) {
     if (o->rows < 0 || o->d <= 0 || o->f <= 0) return OTF_EINVAL;
     // 32-bit element counts of a row tile and of the K extents
     if (o->rows > INT32_MAX / 8 || o->d > (1 << 20) || o->f > (1 << 20)) return OTF_EUNSUPPORTED;
-    // and 32-bit thread counts of the launches
+    // and 32-bit thread counts of the products' launches (the copies of operands, up to five in one, count theirs in two dimensions)
     const int64_t wide = o->d > o->f ? o->d : o->f, most = (int64_t)1 << 34;
     if (o->d * o->f > most || o->rows * wide > most) return OTF_EUNSUPPORTED;
     return OTF_OK;

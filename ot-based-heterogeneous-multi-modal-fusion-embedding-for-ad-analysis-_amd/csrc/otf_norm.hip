@@ -82,11 +82,6 @@ template <int TPR> __device__ __forceinline__ float row_lanes_sum(float x) {
     return x;
 }
 
-// A launch's workgroups, more than 2^20 of them in rows of 2^20: HIP counts a dimension's threads in
-// 32 bits.
-__device__ __forceinline__ int64_t block_id() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
-dim3 blocks(int64_t n) { return n <= 1 << 20 ? dim3((unsigned)n) : dim3(1u << 20, (unsigned)((n + (1 << 20) - 1) >> 20)); }
-
 // Sum of NV values over the TPR threads of a row.  Up to 64: within a wave, no LDS.  Else one
 // barrier: `red` holds two generations of [wave][NV], and a wave can be at most one
 // reduction ahead of another.

@@ -69,6 +69,12 @@ inline bool drop_params(double p, uint32_t& threshold, float& scale) {
     return true;
 }
 
+// ---- launches ---------------------------------------------------------------------------
+// Workgroups, more than 2^20 of them in rows of 2^20: HIP counts a dimension's threads in 32 bits,
+// and launches what is left of a larger count without an error.
+__device__ __forceinline__ int64_t block_id() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+inline dim3 blocks(int64_t n) { return n <= 1 << 20 ? dim3((unsigned)n) : dim3(1u << 20, (unsigned)((n + (1 << 20) - 1) >> 20)); }
+
 // ---- eight consecutive elements of a row, in float ------------------------------------
 // Rows may start at any element: the vector is aligned to its element only (global memory
 // takes unaligned 16-byte accesses on this target), so odd widths and strides keep wide
