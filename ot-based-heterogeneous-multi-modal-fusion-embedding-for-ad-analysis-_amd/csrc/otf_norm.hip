@@ -568,19 +568,19 @@ __global__ __launch_bounds__(256) void norm_param_long_kernel(NormArgs a) {
     norm_param_columns<T, TR, DROP, 4>(a, blockIdx.x, blockIdx.y, gridDim.y);
 }
 
-// partial [groups][2][cols] -> dw (blockIdx.y = 0), db (1).  64 columns a workgroup, its 16
+// partial [groups][2][cols] -> dw (blockIdx.z = 0), db (1).  64 columns a workgroup, its 16
 // waves every 16th partial each, joined in wave order.
 template <typename TW>
 __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restrict__ partial, int groups, int cols,
                                                           TW* dw, TW* db) {
     __shared__ float comb[16 * 64];
-    TW* out = blockIdx.y ? db : dw;
+    TW* out = blockIdx.z ? db : dw;
     if (!out) return;
     const int t = threadIdx.x & 63, wid = threadIdx.x >> 6;
-    const int64_t col = (int64_t)blockIdx.x * 64 + t;
+    const int64_t col = block_id() * 64 + t;
     float s = 0.0f;
     if (col < cols) {
-        const float* p = partial + (int64_t)blockIdx.y * cols + col;
+        const float* p = partial + (int64_t)blockIdx.z * cols + col;
 #pragma unroll 4
         for (int g = wid; g < groups; g += 16) s += p[(int64_t)g * 2 * cols];
     }
@@ -594,6 +594,13 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restric
 }
 
 // ------------------------------------------------------------------------------ dispatch
+template <typename TW> hipError_t norm_param(const float* partial, int groups, int cols, void* dw, void* db, hipStream_t s) {
+    dim3 g = blocks(((int64_t)cols + 63) / 64);
+    g.z = 2;
+    norm_param_kernel<TW><<<g, 1024, 0, s>>>(partial, groups, cols, (TW*)dw, (TW*)db);
+    return hipGetLastError();
+}
+
 template <typename T, typename TR, bool DROP>
 hipError_t norm_forward(const NormArgs& a, hipStream_t s) {
 #define OTF_NF(TPR, CH) norm_forward_kernel<T, TR, DROP, TPR, CH><<<grid, TPR > 256 ? TPR : 256, 0, s>>>(a)
@@ -672,14 +679,9 @@ hipError_t norm_backward_wg(const NormArgs& a, hipStream_t s) {
         if (WG) norm_param_long_kernel<T, TR, DROP><<<dim3((unsigned)((c - 1) / 512 + 1), (unsigned)grid), 256, 0, s>>>(a);
     }
 #undef OTF_NB
-    if (WG && !few && grid > 1) {
-        const dim3 g((unsigned)((c + 63) / 64), 2);
-        if (a.wf32)
-            norm_param_kernel<float><<<g, 1024, 0, s>>>(a.partial, grid, c, (float*)a.dw, (float*)a.db);
-        else
-            norm_param_kernel<T><<<g, 1024, 0, s>>>(a.partial, grid, c, (T*)a.dw, (T*)a.db);
-    }
-    return hipGetLastError();
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !WG || few || grid == 1) return e;
+    return a.wf32 ? norm_param<float>(a.partial, grid, c, a.dw, a.db, s) : norm_param<T>(a.partial, grid, c, a.dw, a.db, s);
 }
 
 template <typename T, typename TR, bool DROP>
@@ -824,14 +826,9 @@ static int norm_backward_call(NormArgs& a, bool drop, int32_t dtype, int32_t rdt
     hipStream_t s = (hipStream_t)stream;
     if (!elem_aligned(a.dw, wdtype) || !elem_aligned(a.db, wdtype) || !elem_aligned(a.w, wdtype)) return OTF_EINVAL;
     if (rows == 0) {   // no row: the sums are zero
-        const int n = (int)cols;
-        const dim3 g((unsigned)((n + 63) / 64), 2);
         if (!a.dw && !a.db) return OTF_OK;
-        if (a.wf32)
-            norm_param_kernel<float><<<g, 1024, 0, s>>>(nullptr, 0, n, (float*)a.dw, (float*)a.db);
-        else
-            norm_param_kernel<_Float16><<<g, 1024, 0, s>>>(nullptr, 0, n, (_Float16*)a.dw, (_Float16*)a.db);  // 0 is 0 in both 16-bit types
-        return check_hip(hipGetLastError());
+        // 0 is 0 in both 16-bit types
+        return check_hip(a.wf32 ? norm_param<float>(nullptr, 0, (int)cols, a.dw, a.db, s) : norm_param<_Float16>(nullptr, 0, (int)cols, a.dw, a.db, s));
     }
     if (!a.x || !a.dy || !a.y || !a.mean || !a.rstd || a.ldx < cols || a.lddy < cols || a.ldy < cols) return OTF_EINVAL;
     if (!elem_aligned(a.x, rdtype) || !elem_aligned(a.dy, dtype) || !elem_aligned(a.y, dtype) ||

@@ -23,3 +23,23 @@ def test_gated_feed_forward_copies_past_32_bit_thread_counts(dev):
     _within(y, want, (half(t) + f * U) * want)
     del flat, y
     torch.cuda.empty_cache()
+
+
+def test_layer_norm_parameter_gradients_past_32_bit_thread_counts(dev):
+    """Rows of more than 2^28 columns: none of them, and 65, whose sums two workgroups a column block
+    share.  x is 1 in the first half of a row and -1 in the second, so mean 0, variance 1, and with
+    dy = 1 a weight's gradient is 65 x / sqrt(1 + eps), 65 or -65 in bfloat16, a bias's 65."""
+    from otfuse import layers
+    rows, cols, t = 65, (1 << 28) + 64, torch.bfloat16
+    w = torch.ones(cols, dtype=t, device=dev, requires_grad=True)
+    none = torch.zeros(0, cols, dtype=t, device=dev)
+    (dw,) = torch.autograd.grad(layers.layer_norm(none, w), w, none)
+    assert torch.count_nonzero(dw) == 0
+    b = torch.zeros(cols, dtype=t, device=dev, requires_grad=True)
+    x = torch.ones(rows, cols, dtype=t, device=dev)
+    x[:, cols // 2:] = -1
+    y = layers.layer_norm(x, w, b)
+    dw, db = torch.autograd.grad(y, (w, b), torch.ones((), dtype=t, device=dev).expand(rows, cols))
+    assert torch.equal(dw, x[0] * 65) and bool((db == 65).all())
+    del none, x, y, dw, db, w, b
+    torch.cuda.empty_cache()
