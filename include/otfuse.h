@@ -658,7 +658,8 @@ int otf_dropout_add_layer_norm_backward(const void* dy, int64_t lddy, const void
 /* ------------------------------------------------------------------------------------
  * Gated feed-forward block: y = (act(x w_gate^T) * (x w_up^T)) w_down^T, and its backward
  * pass.  x, y: (rows, d); w_gate, w_up: (f, d); w_down: (d, f); all of one dtype, float32
- * accumulation.  Weights' leading dimension: at most 2^20, d and f too.
+ * accumulation.  d, f and the leading dimensions of x, dy and the weights: at most 2^20 (also of a single
+ * row, which may name its columns as leading dimension).
  *
  * saved: what backward needs of the forward call (the gate and up products and h), opaque,
  *   otf_gated_ffn_saved_size bytes, 16-byte aligned; NULL in inference.  workspace: 16-byte

@@ -48,7 +48,8 @@ Tensor rows_of(const Tensor& t, int64_t cols) {
     const Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
     return r.stride(1) == 1 && r.stride(0) >= cols ? r : r.contiguous();
 }
-int64_t ld(const Tensor& t) { return t.defined() ? std::max(t.stride(0), t.size(1)) : 0; }
+// A single row has no leading dimension, whatever its stride (contiguous() keeps any): its columns.
+int64_t ld(const Tensor& t) { return !t.defined() ? 0 : t.size(0) <= 1 ? t.size(1) : std::max(t.stride(0), t.size(1)); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 Tensor dense(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }

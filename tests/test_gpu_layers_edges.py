@@ -8,6 +8,50 @@ from test_gpu_layers import T, U, _randn, _within, half
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------ one row, wherever it lies
+def _far_row(t):
+    """t's one row at the end of a sequence of 2^21 elements: torch counts any stride of a single row as
+    contiguous, so nothing makes it dense"""
+    cols = t.shape[1]
+    seq = torch.zeros(1, (1 << 21) // cols + 2, cols, dtype=t.dtype, device=t.device)
+    row = seq[:, -1].copy_(t)
+    assert row.stride(0) > 1 << 20 and row.is_contiguous()
+    return row
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d,f", [(96, 120), (200, 1), (1, 77)])
+def test_gated_feed_forward_of_one_far_row(dev, dt, d, f):
+    """The last token of a long sequence, its gradient, and weights of one row."""
+    from otfuse import layers
+    t = T[dt]
+    x, dy = (_randn(dev, i, 1, d, dtype=t) for i in (1, 5))
+    w = [_randn(dev, i, *s, dtype=t, scale=s[1] ** -0.5) for i, s in ((2, (f, d)), (3, (f, d)), (4, (d, f)))]
+    dense = [v.clone().requires_grad_(True) for v in (x, *w)]
+    want = layers.gated_feed_forward(*dense)
+    want_grads = torch.autograd.grad(want, dense, dy)
+    far = [_far_row(v).requires_grad_(True) if v.shape[0] == 1 else v.clone().requires_grad_(True) for v in (x, *w)]
+    got = layers.gated_feed_forward(*far)
+    assert torch.equal(got, want)
+    for g, h in zip(torch.autograd.grad(got, far, _far_row(dy)), want_grads):
+        assert torch.equal(g, h)
+    with torch.no_grad():
+        assert torch.equal(layers.gated_feed_forward(*far), want)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_row_layers_of_one_far_row(dev, dt):
+    from otfuse import layers
+    x, dy = (_randn(dev, i, 1, 300, dtype=T[dt]) for i in (1, 2))
+    rng = layers.rng_state(3, 4, dev)
+    for call in (lambda v: layers.dropout(v, 0.3, rng, residual=v), layers.layer_norm,
+                 lambda v: layers.dropout_add_layer_norm(v, v, p=0.3, rng=rng)[0]):
+        near, far = x.clone().requires_grad_(True), _far_row(x).requires_grad_(True)
+        y, z = call(near), call(far)
+        assert torch.equal(y, z)
+        assert torch.equal(torch.autograd.grad(y, near, dy)[0], torch.autograd.grad(z, far, _far_row(dy))[0])
+
+
 # ------------------------------------------------------------------ launches past 2^32 threads
 def test_gated_feed_forward_copies_past_32_bit_thread_counts(dev):
     """Three unaligned weights of 1.3e10 elements: their copies are 4.9e9 groups of eight, one launch.
