@@ -222,6 +222,7 @@ template <typename T> __device__ __forceinline__ f32x4 load4(const T* p) {
     return f32x4{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
 }
 
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 // A hidden value in 32 bits but for the last: the value's rounding to T, and `low` elements on what
 // that left out (nothing of an overflow).  low = 0: the rounding alone.
 template <typename T> __device__ __forceinline__ void store_hidden(T* p, int64_t low, f32x4 v) {
@@ -231,7 +232,7 @@ template <typename T> __device__ __forceinline__ void store_hidden(T* p, int64_t
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float high = (float)(T)v[j];
-                v[j] = fabsf(high) < __builtin_inff() ? v[j] - high : 0.0f;
+                v[j] = finite(high) ? v[j] - high : 0.0f;
             }
             store4(p + low, 4, true, v);
         }
@@ -366,11 +367,16 @@ template <typename T, int R> __device__ __forceinline__ uint32_t tr_address(cons
            (((r0 / 8 + ((i & 3) >> 1)) ^ swz_t<T, R>(k)) << 4) + (i & 1) * 8;
 }
 
-// a lane's sums of the rows `low` further on in its 16 (those of the low parts)
-__device__ __forceinline__ f32x4 low_rows(f32x4 v, int low) {
+// A lane's sums with those of the rows `low` further on in its 16 (the low parts').  A sum that is not
+// finite stands alone, as with more rows: an infinite factor meets both parts, and times the low one
+// is an infinity of its sign or, where it is 0, NaN.
+__device__ __forceinline__ f32x4 with_low_rows(f32x4 v, int low) {
     f32x4 r;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = __shfl(v[j], ((int)threadIdx.x & 48) | (((int)threadIdx.x + low) & 15));
+    for (int j = 0; j < 4; ++j) {
+        const float l = __shfl(v[j], ((int)threadIdx.x & 48) | (((int)threadIdx.x + low) & 15));
+        r[j] = finite(v[j]) ? v[j] + l : v[j];
+    }
     return r;
 }
 
@@ -498,7 +504,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& a, int id, int z, int 
             f32x4 r0 = acc[0][0][j][i], r1 = acc[0][1][j][i];
             if constexpr (SUMS == 2) r0 += acc[1][0][j][i], r1 += acc[1][1][j][i];
             if constexpr (TM == 16 && EPI == kStore && sizeof(T) == 2) {
-                if (a.low) r0 += low_rows(r0, a.low), r1 += low_rows(r1, a.low);
+                if (a.low) r0 = with_low_rows(r0, a.low), r1 = with_low_rows(r1, a.low);
             }
             finish4<T, EPI>(a, z, split, m, n, n + TH, r0, r1);
         }
@@ -783,7 +789,7 @@ __global__ __launch_bounds__(64 * NW) void ffn_few_kernel(const T* __restrict__ 
         for (int w = 1; w < NW; ++w) s[b] += part[w][b][lane];
     }
     if constexpr (!GATED && sizeof(T) == 2) {
-        if (low) s[0] += low_rows(s[0], low);
+        if (low) s[0] = with_low_rows(s[0], low);
     }
     if (!live) return;
     const int n = n0 + kc * 4;
@@ -924,15 +930,38 @@ template <typename T> __global__ __launch_bounds__(256) void ffn_outer_mfma_kern
     for (int x = 0; x < 8; ++x) b[x] = four((const T*)j.b, j.ldb, j.low_b, c0 + (x >> 1) * 32 + (i >> 2) * 8 + (x & 1) * 4 + (i & 3), j.C);
     const int col = c0 + q * 8, last = min(j.R, r0 + o.walk * 16);
     typename Outer<T>::type a = four((const T*)j.a, j.lda, j.low_a, r0 + i, j.R);
+    // a fragment without its low terms
+    auto high = [&](typename Outer<T>::type v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (q * 4 + e >= o.rows) v[e] = (T)0.0f;
+        return v;
+    };
     for (int r = r0; r < last; r += 16) {
         const typename Outer<T>::type now = a;
         a = four((const T*)j.a, j.lda, j.low_a, r + 16 + i, last);
         float v[4][8];
+        float bad = 0.0f;   // NaN where one of this lane's sums is not finite
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
             const f32x4 s = Outer<T>::mma(b[x], now);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[x >> 1][(x & 1) * 4 + e] = s[e];
+            for (int e = 0; e < 4; ++e) {
+                v[x >> 1][(x & 1) * 4 + e] = s[e];
+                bad = __builtin_fmaf(s[e], 0.0f, bad);
+            }
+        }
+        // with_low_rows' rule: a sum that is not finite is that of the high parts alone
+        if (terms > o.rows && __any(bad != bad)) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const f32x4 s = Outer<T>::mma(high(b[x]), high(now));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float& w = v[x >> 1][(x & 1) * 4 + e];
+                    w = finite(w) ? w : s[e];
+                }
+            }
         }
         if (r + i >= last) continue;
         T* c = (T*)j.c + (int64_t)(r + i) * j.ldc + col;
@@ -1187,7 +1216,7 @@ hipError_t run_pair(const Product& p, const Product& second, const Pair& q, floa
 // Up to 8 rows of 16-bit operands: the hidden values (h, dg, du) keep their low parts, as many more
 // rows that a 16-row tile has room for, so that only the results are rounded (y of one token 1.0
 // instead of 1.4 times its rounding off).  More rows would cost MFMAs and passes over the hidden
-// values.  A weight or gradient that is infinite meets both parts, and can give NaN for infinity.
+// values.
 int low_rows_of(int64_t rows, int es) { return es == 2 && rows <= 8 ? (int)rows : 0; }
 // The block's buffers and products.  Built twice: for the sizes (null pointers) and to run.
 struct Block {

@@ -52,6 +52,41 @@ def test_row_layers_of_one_far_row(dev, dt):
         assert torch.equal(torch.autograd.grad(y, near, dy)[0], torch.autograd.grad(z, far, _far_row(dy))[0])
 
 
+# ------------------------------------------------------------------ infinities
+def _same_kind(got, want, name):
+    """NaN where the 64-bit form has NaN, the same infinity where it has one, else finite"""
+    got, want = got.detach().double().cpu(), want.cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), name
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf]), name
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("rows,d,f", [(1, 72, 104), (4, 72, 104), (5, 72, 104), (8, 72, 104), (9, 72, 104), (16, 72, 104), (40, 72, 104),
+                                     (8, 2048, 4104), (5, 2050, 4100), (3, 2048, 5632)])
+@pytest.mark.parametrize("where", ["w_down", "w_up", "dy"])
+def test_gated_feed_forward_infinities_do_not_depend_on_the_row_count(dev, dt, rows, d, f, where):
+    """An infinite weight or gradient gives what the formula gives of it: an infinity where one term is
+    infinite, not the difference of two that a value's parts would make."""
+    from otfuse import layers
+    t = T[dt]
+    x = _randn(dev, 1, rows, d, dtype=t)
+    w = [_randn(dev, i, *s, dtype=t, scale=s[1] ** -0.5) for i, s in ((2, (f, d)), (3, (f, d)), (4, (d, f)))]
+    dy = _randn(dev, 5, rows, d, dtype=t)
+    if where == "w_down":
+        w[2][3, 7], w[2][d - 1, f - 1] = float("inf"), float("-inf")
+    elif where == "w_up":
+        w[1][f - 1, 5] = float("inf")
+    else:
+        dy[rows - 1, 2] = float("-inf")
+    args = [v.requires_grad_(True) for v in (x, *w)]
+    y = layers.gated_feed_forward(*args)
+    got = (y, *torch.autograd.grad(y, args, dy))
+    ref = plain.gated_feed_forward(*(v.detach().double().cpu() for v in args), "silu", dy.double().cpu())
+    for name, g, r in zip(("y", "dx", "dw_gate", "dw_up", "dw_down"), got, ref):
+        _same_kind(g, r, name)
+
+
 # ------------------------------------------------------------------ launches past 2^32 threads
 def test_gated_feed_forward_copies_past_32_bit_thread_counts(dev):
     """Three unaligned weights of 1.3e10 elements: their copies are 4.9e9 groups of eight, one launch.
