@@ -87,6 +87,35 @@ def test_gated_feed_forward_infinities_do_not_depend_on_the_row_count(dev, dt, r
         _same_kind(g, r, name)
 
 
+# ------------------------------------------------------------------ the activation's tail
+@pytest.mark.parametrize("dt,low,scale", [("bf16", -12.0, 1.0), ("f16", -5.5, 1024.0)])
+@pytest.mark.parametrize("rows", [4, 12, 40])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_activation_tail(dev, dt, low, scale, rows, act):
+    """act(g) and act'(g) one by one: the gate's weights pick a column of x each, the up product is
+    `scale`, the down product copies.  So y is act(g) scale and dx act'(g) scale of one rounding to
+    the type, up to the float32 evaluation: an exponential of at most 104 powers of two whose argument is
+    seven roundings off, 104 * 7 * 2^-24 * ln 2 = 3e-5 of the value, and a few more: 2^-14."""
+    from otfuse import layers
+    t, n = T[dt], 63
+    g = torch.linspace(low, 6.0, rows * n, dtype=torch.float64).view(rows, n).to(t)
+    x = torch.ones(rows, n + 1, dtype=t)
+    x[:, :n] = g
+    eye = torch.zeros(n, n + 1, dtype=t)
+    eye[:, :n] = torch.eye(n, dtype=t)
+    up = torch.zeros(n, n + 1, dtype=t)
+    up[:, n] = scale
+    args = [v.to(dev) for v in (x, eye, up, eye.t().contiguous())]
+    leaf = args[0].requires_grad_(True)
+    y = layers.gated_feed_forward(*args, activation=act)
+    (dx,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    gd = g.double()
+    value, slope = plain.act(gd, act)
+    _within(y[:, :n], value * scale, (half(t) + 2.0 ** -14) * value.abs() * scale)
+    terms = slope.abs() + 2 * (gd * torch.exp(-gd * gd / 2) / 2.5).abs() if act == "gelu" else slope.abs() + (value * (1 - torch.sigmoid(gd))).abs() * 2
+    _within(dx[:, :n], slope * scale, scale * (half(t) * slope.abs() + 2.0 ** -14 * terms))
+
+
 # ------------------------------------------------------------------ launches past 2^32 threads
 def test_gated_feed_forward_copies_past_32_bit_thread_counts(dev):
     """Three unaligned weights of 1.3e10 elements: their copies are 4.9e9 groups of eight, one launch.
