@@ -8,6 +8,7 @@
 // 16 us, 7 with the checks in Python.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "otfuse.h"
@@ -63,11 +64,21 @@ std::string text(const Tensor& t) {
     o << t.sizes() << " " << t.scalar_type();
     return o.str();
 }
+// What the kernels would drop without a word: a tangent of forward-mode differentiation, and themselves
+// from a trace, which would hold the allocation of the results alone (RuntimeError)
+void plain(const Tensor& t, const char* name) {
+    if (t.defined() && t._fw_grad(/*level=*/0).defined())
+        throw OtfFailure(std::string(name) + " carries a forward-mode tangent: the layers have reverse mode only");
+}
+void no_trace() {
+    if (torch::jit::tracer::isTracing()) throw OtfFailure("the layers cannot be traced: a trace would not hold their kernels");
+}
 void input(const Tensor& t, const char* name) {
     if (!t.defined() || !t.is_cuda()) throw py::type_error(std::string(name) + " must be a ROCm device tensor");
     const auto k = t.scalar_type();
     if (k != at::kFloat && k != at::kHalf && k != at::kBFloat16)
         throw py::type_error(std::string(name) + ": float32, bfloat16 or float16, not " + text(t));
+    plain(t, name);
 }
 void beside(const Tensor& x, const Tensor& t, const char* name) {
     if (t.device() != x.device()) throw py::value_error(std::string(name) + " is not on x's device");
@@ -135,6 +146,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         return dropout_call(x, value(residual), p, rng);
     }
     static variable_list backward(AutogradContext* ctx, variable_list dy) {
+        plain(dy[0], "a gradient");
         const auto rng = ctx->get_saved_variables()[0];
         variable_list g(4);
         if (ctx->saved_data["x"].toBool()) g[0] = dropout_call(dy[0], Tensor(), ctx->saved_data["p"].toDouble(), rng);
@@ -144,6 +156,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(const Tensor& x, double p, const Tensor& rng, const OptTensor& residual) {
+    no_trace();
     input(x, "x");
     if (residual.has_value()) {
         input(*residual, "residual");
@@ -204,6 +217,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         return layer_norm_call(x, weight, bias, eps, x2, stats);
     }
     static variable_list backward(AutogradContext* ctx, variable_list dy) {
+        plain(dy[0], "a gradient");
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &stats = saved[2];
         const int64_t cols = x.size(-1);
@@ -222,6 +236,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    no_trace();
     input(x, "x");
     norm_params(x, weight, bias);
     epsilon(eps);
@@ -275,6 +290,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
         Tensor dy = d[0];
         const Tensor dz = d[1];
         if (!dy.defined() && !dz.defined()) return variable_list(7);
+        for (const Tensor& g : d) plain(g, "a gradient");
         const auto saved = ctx->get_saved_variables();
         const Tensor &stats = saved[1], &rng = saved[2];
         const auto xtype = (at::ScalarType)ctx->saved_data["xtype"].toInt(), rtype = (at::ScalarType)ctx->saved_data["rtype"].toInt();
@@ -302,6 +318,7 @@ struct AddNorm : torch::autograd::Function<AddNorm> {
 
 std::pair<Tensor, Tensor> dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const OptTensor& weight,
                                                  const OptTensor& bias, double p, const OptTensor& rng, double eps) {
+    no_trace();
     input(x, "x");
     input(residual, "residual");
     beside(x, residual, "residual");
@@ -371,6 +388,7 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        plain(grads[0], "a gradient");
         const auto s = ctx->get_saved_variables();
         const Tensor &x = s[0], &dy = grads[0];
         const c10::DeviceGuard guard(x.device());
@@ -392,6 +410,7 @@ struct GatedFeedForward : torch::autograd::Function<GatedFeedForward> {
 };
 
 Tensor gated_feed_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const std::string& activation) {
+    no_trace();
     input(x, "x");
     const std::pair<const Tensor*, const char*> weights[3] = {{&wg, "w_gate"}, {&wu, "w_up"}, {&wd, "w_down"}};
     for (const auto& [t, name] : weights) {

@@ -14,8 +14,9 @@ Tensors live on a ROCm device; kernels run on the current stream of the tensors'
 nothing synchronises, so every call can be captured into a graph: forward and backward together,
 and with no eager graph of the same leaves alive (autograd runs a node on the stream that its
 forward, or a leaf's first use in a graph that lives, ran on).  Inputs are float32, bfloat16 or
-float16; statistics and sums are float32.  Each function takes part in autograd;
-without a gradient to compute, nothing is kept for backward.
+float16; statistics and sums are float32.  Each function takes part in autograd, in reverse
+mode and once: second derivatives, forward-mode tangents, tracing and function transforms are refused.
+Without a gradient to compute, nothing is kept for backward.
 """
 from __future__ import annotations
 

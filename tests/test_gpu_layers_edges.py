@@ -116,6 +116,61 @@ def test_activation_tail(dev, dt, low, scale, rows, act):
     _within(dx[:, :n], slope * scale, scale * (half(t) * slope.abs() + 2.0 ** -14 * terms))
 
 
+# ------------------------------------------------------------------ what is refused
+def _calls(dev):
+    from otfuse import layers
+    rng = layers.rng_state(1, 2, dev)
+    w, b = torch.ones(16, device=dev), torch.zeros(16, device=dev)
+    wi, wo = torch.ones(24, 16, device=dev), torch.ones(16, 24, device=dev)
+    return {"dropout": lambda x: layers.dropout(x, 0.1, rng), "dropout residual": lambda x: layers.dropout(torch.ones_like(w).expand(4, 16), 0.1, rng, residual=x),
+            "layer_norm": lambda x: layers.layer_norm(x, w, b), "add_norm": lambda x: layers.dropout_add_layer_norm(x, torch.ones(4, 16, device=dev), w, b)[0],
+            "add_norm residual": lambda x: layers.dropout_add_layer_norm(torch.ones(4, 16, device=dev), x, w, b)[0],
+            "ffn": lambda x: layers.gated_feed_forward(x, wi, wi, wo)}
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_is_refused(dev, leaf):
+    """A tangent that the kernels do not carry on is an error, not a constant."""
+    import torch.autograd.forward_ad as fwad
+    from otfuse import layers
+    x = torch.randn(4, 16, device=dev).requires_grad_(leaf)
+    for name, call in _calls(dev).items():
+        with fwad.dual_level():
+            with pytest.raises(RuntimeError, match="forward"):
+                call(fwad.make_dual(x, torch.ones(4, 16, device=dev)))
+        call(x)
+    v, m = torch.ones(16, device=dev), torch.ones(24, 16, device=dev)
+    with fwad.dual_level():
+        for call in (lambda: layers.layer_norm(x, fwad.make_dual(v, v)), lambda: layers.layer_norm(x, None, fwad.make_dual(v, v)),
+                     lambda: layers.dropout_add_layer_norm(x, x, fwad.make_dual(v, v)),
+                     lambda: layers.gated_feed_forward(x, fwad.make_dual(m, m), m, m.t()),
+                     lambda: layers.gated_feed_forward(x, m, fwad.make_dual(m, m), m.t()),
+                     lambda: layers.gated_feed_forward(x, m, m, fwad.make_dual(m, m).t())):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        if leaf:   # a tangent that reaches backward alone
+            for call in _calls(dev).values():
+                for y in call(x), *layers.dropout_add_layer_norm(x, x):
+                    with pytest.raises(RuntimeError, match="forward"):
+                        torch.autograd.grad((y * fwad.make_dual(torch.ones_like(y), torch.ones_like(y))).sum(), x)
+
+
+def test_tracing_and_transforms_are_refused(dev):
+    """A trace would hold the results' allocation without the kernels that fill them; a transform's
+    wrapped tensors have no memory to read."""
+    x = torch.randn(4, 16, device=dev)
+    for name, call in _calls(dev).items():
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (x,))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.expand(3, 4, 16))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(x)
+        call(x)
+
+
 # ------------------------------------------------------------------ launches past 2^32 threads
 def test_gated_feed_forward_copies_past_32_bit_thread_counts(dev):
     """Three unaligned weights of 1.3e10 elements: their copies are 4.9e9 groups of eight, one launch.
