@@ -241,6 +241,7 @@ def ptr(t) -> int | None:
 
 
 def stream_handle(device=None) -> int:
-    """The current stream of `device` (a torch.device with an index, or None: the current one)."""
-    index = getattr(device, "index", None)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+    """The current stream of `device` (a torch.device, its name or its index; None: the current one)."""
+    if isinstance(device, torch.device) and device.type == "cuda" and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)   # a tensor's device: without a stream object
+    return torch.cuda.current_stream(device).cuda_stream
