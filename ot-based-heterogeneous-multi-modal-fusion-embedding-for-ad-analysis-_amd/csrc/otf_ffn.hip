@@ -1326,7 +1326,8 @@ struct Saved {
     float *g, *u;
     char* h;
 };
-Saved carve_saved(void* p, int64_t n, int64_t fk, int es) {
+Saved carve_saved(void* p, int64_t n, int64_t fk) {
+    if (!p) return Saved{};   // a size query
     char* b = (char*)p;
     const size_t wide = up256((size_t)(n * fk) * 4);
     return Saved{(float*)b, (float*)(b + wide), b + 2 * wide};
@@ -1340,7 +1341,7 @@ template <typename T> int forward(const otf_ffn_args* o, void* workspace, size_t
     Block b(o, (int)sizeof(T), workspace);
     Saved sv{};
     if (o->saved)
-        sv = carve_saved(o->saved, b.n, b.fk, b.es);
+        sv = carve_saved(o->saved, b.n, b.fk);
     else
         sv.h = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
     if (few_rows(b.n, b.d, b.f, b.es)) {
@@ -1420,7 +1421,7 @@ hipError_t run_outer(const Block& b, const char* dg, const char* du, const char*
 
 template <typename T> int backward(const otf_ffn_args* o, void* workspace, size_t* need, const size_t* have, hipStream_t s) {
     Block b(o, (int)sizeof(T), workspace);
-    const Saved sv = carve_saved(o->saved, b.n, b.fk, b.es);
+    const Saved sv = carve_saved(o->saved, b.n, b.fk);
     const bool win = o->dw_gate != nullptr, wdown = o->dw_down != nullptr, wx = o->dx != nullptr;
     char* dg = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
     char* du = (char*)b.ws.take((size_t)(b.nh * b.fk * b.es));
