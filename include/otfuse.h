@@ -686,6 +686,7 @@ typedef struct {
     void* dw_up;         int64_t lddw_in;
     void* dw_down;       int64_t lddw_down;
 } otf_ffn_args;
+/* The sizes of what no call takes are 0. */
 size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype);
 size_t otf_gated_ffn_workspace_size(const otf_ffn_args* args);
 int otf_gated_ffn(const otf_ffn_args* args, void* workspace, size_t workspace_bytes, otf_stream_t stream);

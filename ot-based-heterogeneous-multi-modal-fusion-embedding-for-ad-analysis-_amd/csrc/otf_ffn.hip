@@ -1306,16 +1306,19 @@ bool few_rows(int64_t rows, int64_t d, int64_t f, int es) {
     return rows <= 16 && (es == 4 || rows * d * f <= (int64_t)1 << 26);
 }
 
+constexpr int64_t kMaxRows = INT32_MAX / 8, kMaxWidth = 1 << 20, kMaxElements = (int64_t)1 << 34;
+bool is_type(int32_t t) { return t == OTF_F32 || t == OTF_F16 || t == OTF_BF16; }
+
 int check_ffn(const otf_ffn_args* o) {
     if (!o) return OTF_EINVAL;
-    if (o->dtype != OTF_F32 && o->dtype != OTF_F16 && o->dtype != OTF_BF16) return OTF_EINVAL;
+    if (!is_type(o->dtype)) return OTF_EINVAL;
     if (o->activation != OTF_ACT_SILU && o->activation != OTF_ACT_GELU) return OTF_EINVAL;
     if (o->rows < 0 || o->d <= 0 || o->f <= 0) return OTF_EINVAL;
     // 32-bit element counts of a row tile and of the K extents
-    if (o->rows > INT32_MAX / 8 || o->d > (1 << 20) || o->f > (1 << 20)) return OTF_EUNSUPPORTED;
+    if (o->rows > kMaxRows || o->d > kMaxWidth || o->f > kMaxWidth) return OTF_EUNSUPPORTED;
     // and 32-bit thread counts of the products' launches (the copies of operands, up to five in one, count theirs in two dimensions)
-    const int64_t wide = o->d > o->f ? o->d : o->f, most = (int64_t)1 << 34;
-    if (o->d * o->f > most || o->rows * wide > most) return OTF_EUNSUPPORTED;
+    const int64_t wide = o->d > o->f ? o->d : o->f;
+    if (o->d * o->f > kMaxElements || o->rows * wide > kMaxElements) return OTF_EUNSUPPORTED;
     return OTF_OK;
 }
 // leading dimensions: 256 rows within a 31-bit byte offset
@@ -1500,7 +1503,8 @@ using namespace otf;
 extern "C" {
 
 size_t otf_gated_ffn_saved_size(int64_t rows, int64_t f, int32_t dtype) {
-    if (rows <= 0 || f <= 0) return 0;
+    if (rows <= 0 || f <= 0 || !is_type(dtype)) return 0;
+    if (rows > kMaxRows || f > kMaxWidth || rows * f > kMaxElements) return 0;   // no call takes them
     return saved_bytes(rows, up_ktile(f, (int)esize(dtype)), (int)esize(dtype));
 }
 

@@ -719,13 +719,15 @@ bool type16_or_32(int32_t t) { return t == OTF_F32 || t == OTF_F16 || t == OTF_B
 size_t elem_size(int32_t t) { return t == OTF_F32 ? 4 : 2; }
 bool elem_aligned(const void* p, int32_t t) { return (uintptr_t)p % elem_size(t) == 0; }
 
-// what every call here checks: sizes within the kernels' index types, types, parameters
+bool too_large(int64_t rows, int64_t cols) { return rows > INT32_MAX || cols > INT32_MAX - 8192; }   // the kernels' index types
+
+// what every call here checks: sizes, types, parameters
 int check_norm(int64_t rows, int64_t cols, int32_t dtype, int32_t rdtype, int32_t wdtype) {
     if (rows < 0 || cols <= 0) return OTF_EINVAL;
     if (!type16_or_32(dtype)) return OTF_EINVAL;
     if (rdtype != dtype && rdtype != OTF_F32) return OTF_EINVAL;
     if (wdtype != dtype && wdtype != OTF_F32) return OTF_EINVAL;
-    if (rows > INT32_MAX || cols > INT32_MAX - 8192) return OTF_EUNSUPPORTED;
+    if (too_large(rows, cols)) return OTF_EUNSUPPORTED;
     return OTF_OK;
 }
 
@@ -811,7 +813,7 @@ int otf_dropout_add_layer_norm(const void* x, int64_t ldx, int32_t dtype, const 
 }
 
 size_t otf_layer_norm_backward_workspace_size(int64_t rows, int64_t cols) {
-    if (rows <= 0 || cols <= 0) return 0;
+    if (rows <= 0 || cols <= 0 || too_large(rows, cols)) return 0;
     if (cols <= kMaxHeldColsBackward && rows <= kFewRows) return 0;
     const int g = norm_backward_groups(rows, cols);
     return g > 1 ? (size_t)g * 2 * (size_t)cols * sizeof(float) : 0;

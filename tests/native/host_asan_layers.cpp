@@ -46,8 +46,10 @@ int main() {
                         const bool taken = d * f <= limit && n * (d > f ? d : f) <= limit;
                         const size_t es = t == OTF_F32 ? 4 : 2;
                         const size_t saved = otf_gated_ffn_saved_size(n, f, t);
-                        if (taken)
+                        if (n * f <= limit)
                             CHECK(saved >= (size_t)(n * f) * (8 + es), "saved %lld x %lld", (long long)n, (long long)f);
+                        else
+                            CHECK(saved == 0, "saved size of what is refused");
                         const size_t kept = otf_gated_ffn_workspace_size(&a);
                         a.saved = nullptr;
                         const size_t infer = otf_gated_ffn_workspace_size(&a);
@@ -72,6 +74,22 @@ int main() {
                         }
                     }
     CHECK(asked > 40000, "sizes swept");
+    // sizes that no call takes
+    const int64_t huge[] = {INT64_MAX, INT64_MAX - 63, (int64_t)1 << 62, (int64_t)1 << 40, -1, 0, INT64_MIN};
+    for (int64_t n : huge)
+        for (int64_t m : huge) {
+            CHECK(otf_gated_ffn_saved_size(n, m, OTF_F32) == 0, "saved %lld %lld", (long long)n, (long long)m);
+            CHECK(otf_gated_ffn_saved_size(n, 8, OTF_BF16) == 0 && otf_gated_ffn_saved_size(8, m, OTF_BF16) == 0, "saved");
+            CHECK(otf_layer_norm_backward_workspace_size(n, m) == 0, "norm %lld %lld", (long long)n, (long long)m);
+            CHECK(otf_layer_norm_backward_workspace_size(n, 8) == 0 && otf_layer_norm_backward_workspace_size(8, m) == 0, "norm");
+            otf_ffn_args a = ffn(n, m, m, OTF_F32, 0);
+            CHECK(otf_gated_ffn_workspace_size(&a) == 0 && otf_gated_ffn_backward_workspace_size(&a) == 0, "workspace");
+            CHECK(n == 0 || otf_gated_ffn(&a, buffer, sizeof buffer, nullptr) != OTF_OK, "call");
+            CHECK(otf_dropout(buffer, n, nullptr, 0, buffer, n, m, n, OTF_F32, 0.5, nullptr, nullptr) != OTF_OK || n == 0 || m == 0, "dropout");
+            CHECK(otf_layer_norm(buffer, n, OTF_F32, nullptr, nullptr, OTF_F32, 1e-5, m, n, buffer, n, nullptr, nullptr, nullptr) != OTF_OK || m == 0,
+                  "norm call");
+        }
+    CHECK(otf_gated_ffn_saved_size(8, 8, 99) == 0, "saved size of no type");
     // rows and columns at the norms' limits
     for (int64_t n : {(int64_t)1, (int64_t)64, (int64_t)65, (int64_t)8191, (int64_t)1 << 24, (int64_t)INT32_MAX})
         for (int64_t c : {(int64_t)1, (int64_t)64, (int64_t)1531, (int64_t)16384, (int64_t)16385, (int64_t)INT32_MAX - 8192}) {
@@ -79,6 +97,7 @@ int main() {
             CHECK(n <= 64 ? ws == 0 : ws >= (size_t)c * 16, "norm workspace %lld x %lld", (long long)n, (long long)c);
             CHECK(ws % ((size_t)c * 8) == 0, "whole partials");
         }
+    CHECK(otf_layer_norm_backward_workspace_size((int64_t)INT32_MAX + 1, 8) == 0, "rows past the limit");
     // refused calls
     otf_ffn_args a = ffn(20, 16, 24, OTF_BF16, 0);
     CHECK(otf_gated_ffn(nullptr, buffer, 4096, nullptr) == OTF_EINVAL && otf_gated_ffn_backward(nullptr, buffer, 4096, nullptr) == OTF_EINVAL, "null");
