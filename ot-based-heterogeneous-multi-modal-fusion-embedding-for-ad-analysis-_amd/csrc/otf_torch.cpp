@@ -44,16 +44,18 @@ otf_stream_t stream_of(const Tensor& t) {
     return (otf_stream_t)c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream();
 }
 
+// a lazily negated view (the imaginary part of a conjugate) as the values that it stands for
+Tensor resolved(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 // (..., cols) -> (rows, cols) with unit column stride and rows that do not overlap
 Tensor rows_of(const Tensor& t, int64_t cols) {
-    const Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
+    const Tensor r = resolved(t.dim() == 2 ? t : t.reshape({-1, cols}));
     return r.stride(1) == 1 && r.stride(0) >= cols ? r : r.contiguous();
 }
 // A single row has no leading dimension, whatever its stride (contiguous() keeps any): its columns.
 int64_t ld(const Tensor& t) { return !t.defined() ? 0 : t.size(0) <= 1 ? t.size(1) : std::max(t.stride(0), t.size(1)); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor value(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
-Tensor dense(const OptTensor& t) { return t.has_value() && t->defined() ? t->contiguous() : Tensor(); }
+Tensor dense(const OptTensor& t) { return t.has_value() && t->defined() ? resolved(*t).contiguous() : Tensor(); }
 const int64_t* words(const Tensor& rng) { return rng.defined() ? rng.const_data_ptr<int64_t>() : nullptr; }
 bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && wants(*t); }

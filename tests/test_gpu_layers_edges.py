@@ -52,6 +52,30 @@ def test_row_layers_of_one_far_row(dev, dt):
         assert torch.equal(torch.autograd.grad(y, near, dy)[0], torch.autograd.grad(z, far, _far_row(dy))[0])
 
 
+# ------------------------------------------------------------------ lazily negated views
+def test_imaginary_parts_of_conjugates(dev):
+    """torch keeps them as a view with a sign to be applied: of one element, or made so by hand, it is
+    contiguous and its memory holds the other sign."""
+    from otfuse import layers
+    rng = layers.rng_state(3, 4, dev)
+    one = torch.complex(*(torch.randn(1, 1, device=dev) for _ in range(2))).conj().imag
+    many = torch._neg_view(torch.randn(20, 72, device=dev))
+    assert one.is_neg() and many.is_neg()
+    for v in (one, many):
+        plain_v, cols = v.resolve_neg().clone(), v.shape[1]
+        w = torch.randn(24, cols, device=dev)
+        for call in (lambda t, s: layers.dropout(t, 0.0, rng, residual=s), lambda t, s: layers.layer_norm(t, t[0], s[0]),
+                     lambda t, s: layers.dropout_add_layer_norm(t, s)[0], lambda t, s: layers.gated_feed_forward(t, w, w, w.t()),
+                     lambda t, s: layers.gated_feed_forward(s, t[:1], s[:1], t[:1].t())):
+            a, b = v.detach().requires_grad_(True), plain_v.clone().requires_grad_(True)
+            assert a.is_neg()
+            y, z = call(a, plain_v), call(b, plain_v)
+            assert torch.equal(y, z)
+            assert torch.equal(*(torch.autograd.grad(o, leaf, torch.ones_like(z))[0] for o, leaf in ((y, a), (z, b))))
+            with torch.no_grad():
+                assert torch.equal(call(v, plain_v), z)
+
+
 # ------------------------------------------------------------------ infinities
 def _same_kind(got, want, name):
     """NaN where the 64-bit form has NaN, the same infinity where it has one, else finite"""
