@@ -440,7 +440,7 @@ __global__ __launch_bounds__(512) void sk_mesh_kernel(SkMeshArgs p) {
     const T ks = (T)(-unit / p.reg * cinv);
 
     // ---- K for this wave's 16 rows x this lane's 8 columns, once (0 outside C), as
-    // pairs of adjacent columns: the row and column partials run on v_pk_fma_f32
+    // pairs of adjacent columns (an FMA each: packed float32 instructions are not emitted)
     F2 kv[R][G][2];
     if constexpr (PW) {
         if (!pw_cost_tile32<R, G>(p, kv, pwb, rb, cb, nrb * ncb, lead, deadline, &pw_flag, pw_wmx,

@@ -177,7 +177,7 @@ __device__ __forceinline__ void widen(const Raw& r, T (&out)[RawN<CT>::N]) {
 
 // 16 B of cost -> pairs of (cost x ks) in the compute type.  fp16 x f32 in one
 // v_fma_mix_f32 per element (the fp16 -> f32 conversion is exact, so this rounds once,
-// exactly like convert-then-multiply), f32 pairs by one v_pk_mul_f32.
+// exactly like convert-then-multiply), f32 pairs by two products.
 template <typename T> using Pair = __attribute__((ext_vector_type(2))) T;
 template <typename T, typename CT>
 __device__ __forceinline__ void scaled_pairs(const Raw& r, T ks, Pair<T> (&out)[RawN<CT>::N / 2]) {
@@ -456,8 +456,7 @@ __global__ __launch_bounds__(kSwNT) void sk_sweep_kernel(SkSweepArgs<T> p) {
     if (tid == 0 && blockIdx.x < 256) g_stamps[(blockIdx.x * 16 + 15) * 8 + 7] = (unsigned long long)xcd;
 #endif
     Raw bufA[R][G];
-    // column partials as pairs of adjacent columns: the e * u products go out as packed
-    // FMAs (v_pk_fma_f32), as do the e * v row-sum products
+    // column partials as pairs of adjacent columns, an FMA each, as the e * v row-sum products
     using T2 = Pair<T>;
     constexpr int VP2 = VC / 2;
     T2 colacc[G][VP2];

@@ -14,9 +14,9 @@ torch.  Here the whole block stays on the device and in HIP kernels:
 
 ``group_features_by_label`` mirrors MRI_PET_OT_nojax.py:884-903 for the per-epoch path.
 
-``FeedForwardBlock`` is the part of SelfAttentionBlock after its attention
+``FeedForwardBlock`` stands in the place of SelfAttentionBlock's part after its attention
 (MRI_PET_OT_nojax.py:523-549) on the kernels of ``layers``: residual sums with dropout and
-layer norm, and a gated feed-forward part between them.
+layer norm, and a gated feed-forward part without biases between them (parity unpinned).
 """
 from __future__ import annotations
 

@@ -8,7 +8,8 @@ MRI_PET_OT_OT_per_epoch_attn.py:963-1065).  Here:
     dropout                  y = [residual +] keep * x / (1 - p), the mask never stored
     layer_norm               with the parameter gradients' reduction
     dropout_add_layer_norm   z = residual + dropout(x), y = LN(z), one pass over the rows
-    gated_feed_forward       (act(x Wg^T) * (x Wu^T)) Wd^T on the matrix cores
+    gated_feed_forward       (act(x Wg^T) * (x Wu^T)) Wd^T on the matrix cores, in the place of the
+                             block's feed-forward part (parity with it unpinned)
 
 Tensors live on a ROCm device; kernels run on the current stream of the tensors' device and
 nothing synchronises, so every call can be captured into a graph: forward and backward together,
@@ -98,6 +99,8 @@ def gated_feed_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
     feed-forward part (MRI_PET_OT_nojax.py:523-549).
 
     x: (..., d); w_gate, w_up: (f, d); w_down: (d, f), as ``torch.nn.Linear`` keeps them, all of
-    x's type.  ``activation``: "silu" or "gelu" (the exact form).  Sums are float32; the hidden
-    activations are rounded to x's type, the two products that backward needs are kept in float32."""
+    x's type.  ``activation``: "silu" or "gelu" (the exact form).  Sums are float32.  The hidden
+    activations and their gradients are rounded to x's type; up to 8 rows of 16-bit types they keep what
+    that leaves out.  For backward the gate and up products are kept in float32 beside the hidden
+    activations: 10 bytes a hidden value of 16-bit types, 12 of float32."""
     return _native().gated_feed_forward(x, w_gate, w_up, w_down, activation)
